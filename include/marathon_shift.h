@@ -71,6 +71,11 @@ extern "C" {
 #define MSHIFT_EBIT_CLAIM 32u   /* the tile-claim counter went backwards (the status word
                                    was shared with a launch in flight); the launch stopped */
 
+/* Set by the serving operators (block maps, rotary, append, attend) in their own *err;
+ * bits 8..31 are not used by those. */
+#define MSHIFT_ERR_LENGTHS 64u /* a length below 0, or past the bound the caller gave */
+#define MSHIFT_ERR_POOL 128u   /* too few free blocks, or a position past its block table */
+
 /* ---- element types ----------------------------------------------------- */
 #define MSHIFT_BF16 0
 #define MSHIFT_F16 1
@@ -270,6 +275,94 @@ MSHIFT_API int mshift_stage(const mshift_copy* copies, int32_t n, void* stream);
  * dereference peer memory: only mshift_stage copies read it.
  */
 MSHIFT_API int mshift_enable_peer(int32_t peer_device);
+
+/*
+ * Serving operators over a paged e4m3 cache with one fp32 scale for each block and
+ * head: element = code * scale[block, head], scales separate for K and V.  The
+ * reference has none of them (its cache is vLLM's own, its requests are planned
+ * on the host).  Common to all four:
+ *   - requests are rows query_start[r] .. query_start[r + 1] of the token axis
+ *     (device int32 [reqs + 1]); seq_lens[r] (device int32) counts the request's
+ *     tokens in the cache including those rows, so row i of request r stands at position
+ *     seq_lens[r] - (its row count) + i;
+ *   - block_tables is int32 [reqs, width] with table_stride elements between rows; an
+ *     entry outside [0, num_blocks) that is needed is not followed and sets MSHIFT_EBIT_SLOT;
+ *   - err is a device word the caller zeroes; the device of `stream` is current.
+ */
+
+/*
+ * Block tables and slot maps of one step from request lengths, in one launch.
+ * Request r holds cached_lens[r] tokens and gets new_lens[r] more; the blocks
+ * it lacks are taken from free_blocks[*free_head ...] in request order and entered
+ * into block_tables.  Written: query_start [reqs + 1], seq_lens [reqs], and for the
+ * `tokens` rows slots (block * block_size + offset) and positions; rows behind the
+ * last request get slot -1, position 0.  free_head_out (not free_head itself) gets the
+ * new head.  Too few free blocks, or a table too narrow: slot -1 and MSHIFT_ERR_POOL.
+ * More new tokens than `tokens`: the surplus is dropped and MSHIFT_ERR_LENGTHS set.
+ */
+MSHIFT_API int mshift_block_maps(const int32_t* cached_lens, const int32_t* new_lens,
+                int32_t reqs, int32_t* block_tables, int64_t table_stride, int32_t width,
+                const int32_t* free_blocks, int32_t free_len, const int32_t* free_head,
+                int32_t block_size, int32_t tokens, int32_t* query_start, int32_t* seq_lens,
+                int64_t* slots, int64_t* positions, int32_t* free_head_out, uint32_t* err,
+                void* stream);
+
+/*
+ * Rotary positions with several axes: frequency i < rotary / 2 of row t turns by
+ * positions[axes[i] * pos_axis_stride + t] * inv_freq[i] (NeoX half-split pairs), by its
+ * negative if `inverse`.  q [n, hq, head_size] and k [n, hk, head_size] of dtype (BF16, F16 or
+ * F32) with element strides; the results go to q_out / k_out, which may be q / k
+ * themselves but not overlap them otherwise.  axes NULL: axis 0.  The angle is exact
+ * modulo a turn to about 2^-24 turns at any position.  An entry of axes outside [0, n_axes)
+ * sets MSHIFT_EBIT_TABLE and reads axis 0.
+ */
+MSHIFT_API int mshift_rotary_axes(int32_t dtype, const void* q, int64_t q_tok, int64_t q_head,
+                void* q_out, int64_t qo_tok, int64_t qo_head, int32_t hq, const void* k,
+                int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
+                int32_t hk, int64_t n, int32_t head_size, int32_t rotary, const void* positions,
+                int64_t pos_axis_stride, int32_t pos_is_64, int32_t n_axes,
+                const float* inv_freq, const int32_t* axes, int32_t inverse, uint32_t* err,
+                void* stream);
+
+/*
+ * Append: rows k, v [rows, heads, head_size] (BF16, F16 or F32) into the cache at
+ * their requests' last positions.  A block that holds earlier tokens of its request keeps
+ * them (requantised if its scale has to grow); one that does not gets its scale from the
+ * new rows alone.  paged->dtype is MSHIFT_E4M3, head_size 64, 128 or 256.  Two requests
+ * of a call must not write the same block.
+ */
+MSHIFT_API int mshift_append_block_scaled(int32_t dtype, const void* k, int64_t k_tok,
+                int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t rows,
+                const mshift_paged* paged, void* k_base, void* v_base, float* k_scale,
+                int64_t ks_blk, int64_t ks_head, float* v_scale, int64_t vs_blk,
+                int64_t vs_head, const int32_t* block_tables, int64_t table_stride,
+                int32_t width, const int32_t* query_start, const int32_t* seq_lens,
+                int32_t reqs, uint32_t* err, void* stream);
+
+/* Bytes of device workspace mshift_attend_block_scaled needs (16-byte aligned), or -1. */
+MSHIFT_API int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk,
+                int32_t head_size, int32_t reqs, int32_t max_query_len, int32_t max_seq_len);
+
+/*
+ * Attention of q [rows, hq, head_size] (BF16 or F16; query head j reads KV head
+ * j / (hq / heads)) over the cache: row at position x sees the keys [0, x] of its request
+ * (all of them without `causal`), and of those the last `window` if window > 0.
+ * out [rows, hq, head_size] of q's dtype; lse [rows, hq] fp32 (natural log) or NULL.
+ * A row that sees no key gets zeros and -inf.  Rows behind the last request are left as they were,
+ * or zeroed if zero_tail.  max_query_len / max_seq_len bound the requests' rows and
+ * lengths; a request past them is cut off there and sets MSHIFT_ERR_LENGTHS.  Keys in
+ * a bad block count as unseen.  Value scales below 2^-64 are read as 2^-64.
+ */
+MSHIFT_API int mshift_attend_block_scaled(int32_t dtype, const void* q, int64_t q_tok,
+                int64_t q_head, int32_t rows, int32_t hq, const mshift_paged* paged,
+                const void* k_base, const void* v_base, const float* k_scale,
+                int64_t ks_blk, int64_t ks_head, const float* v_scale, int64_t vs_blk,
+                int64_t vs_head, const int32_t* block_tables, int64_t table_stride,
+                int32_t width, const int32_t* query_start, const int32_t* seq_lens,
+                int32_t reqs, int32_t max_query_len, int32_t max_seq_len, float scale,
+                int32_t causal, int32_t window, void* out, int64_t o_tok, int64_t o_head,
+                float* lse, int32_t zero_tail, void* workspace, int64_t workspace_bytes,
+                uint32_t* err, void* stream);
 
 #ifdef __cplusplus
 }

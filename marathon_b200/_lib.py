@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libmarathon_shift.so"
 
 OK, EINVAL, EUNSUPPORTED, ECUDA, ETOOBIG = 0, 1, 2, 3, 4
 EBIT_SLOT, EBIT_STORE, EBIT_SESSION, EBIT_TABLE, EBIT_TIMEOUT, EBIT_CLAIM = 1, 2, 4, 8, 16, 32
+ERR_LENGTHS, ERR_POOL = 64, 128
 BF16, F16, F32, E4M3 = 0, 1, 2, 3
 KERNEL_LSU, KERNEL_BULK, KERNEL_AUTO = 0, 1, 2
 
@@ -40,6 +41,11 @@ EXPORTS = (
     "mshift_debug_first_wait",
     "mshift_stage",
     "mshift_enable_peer",
+    "mshift_block_maps",
+    "mshift_rotary_axes",
+    "mshift_append_block_scaled",
+    "mshift_attend_workspace",
+    "mshift_attend_block_scaled",
 )
 
 
@@ -130,6 +136,27 @@ _SIGNATURES = {
     "mshift_debug_first_wait": (_I32, [_I32]),
     "mshift_stage": (ctypes.c_int, [_P, _I32, _P]),
     "mshift_enable_peer": (ctypes.c_int, [_I32]),
+    "mshift_block_maps": (
+        ctypes.c_int,
+        [_P, _P, _I32, _P, _I64, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "mshift_rotary_axes": (
+        ctypes.c_int,
+        [_I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64,
+         _I32, _I32, _P, _I64, _I32, _I32, _P, _P, _I32, _P, _P],
+    ),
+    "mshift_append_block_scaled": (
+        ctypes.c_int,
+        [_I32, _P, _I64, _I64, _P, _I64, _I64, _I32, ctypes.POINTER(Paged), _P, _P, _P, _I64, _I64,
+         _P, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _P],
+    ),
+    "mshift_attend_workspace": (_I64, [_I32] * 7),
+    "mshift_attend_block_scaled": (
+        ctypes.c_int,
+        [_I32, _P, _I64, _I64, _I32, _I32, ctypes.POINTER(Paged), _P, _P, _P, _I64, _I64, _P, _I64,
+         _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, ctypes.c_float, _I32, _I32, _P, _I64, _I64,
+         _P, _I32, _P, _I64, _P, _P],
+    ),
 }
 
 _lock = threading.Lock()
@@ -185,6 +212,8 @@ def describe_bits(bits: int) -> str:
         (EBIT_TIMEOUT, "a bulk copy did not complete in time; the launch stopped early"),
         (EBIT_CLAIM, "the tile-claim counter went backwards (status word shared with a "
                      "launch in flight); the launch stopped early"),
+        (ERR_LENGTHS, "a request length below zero or past the call's bound"),
+        (ERR_POOL, "too few free blocks, or a position past its block table"),
     ):
         if bits & bit:
             names.append(name)

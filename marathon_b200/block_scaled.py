@@ -1,0 +1,199 @@
+"""A paged cache held in 8 bits with a scale for each block of tokens and head.
+
+The shift path's e4m3 caches have one scale a layer, which the caller calibrates.
+Here every block has its own scale for each head, kept beside the cache in two
+fp32 tensors ``k_scale`` and ``v_scale`` of shape ``[blocks, heads]``: an
+element is ``code * scale[block, head]``.  :func:`append_block_scaled` writes new tokens
+and chooses the scales; :func:`attend_block_scaled` is the attention that reads the cache, for decoding,
+chunks and whole prefills in one batch.  The codes lie in any of the paged
+layouts of :mod:`marathon_b200.paged` (``nhd``, ``hnd``, ``split``, ``split_blocks``); head sizes 64, 128 and
+256.
+
+Both take a step as :func:`marathon_b200.block_maps.block_maps` describes it: request ``r`` owns the rows
+``query_start[r]:query_start[r + 1]``, its last row stands at position ``seq_lens[r] - 1``,
+and position ``p`` lies in block ``block_tables[r, p // block_size]``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from ._serve import (
+    Launch, block_table_rows, cuda_on, finish, geometry, heads_rows, int32_vector, overlap,
+    refuse_grad, scale_strides,
+)
+from .paged import base_pointers, dtype_code
+
+__all__ = ["append_block_scaled", "attend_block_scaled"]
+
+HEAD_SIZES = (64, 128, 256)
+
+
+def _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size, layout):
+    """Checks what both operators take; (geometry, its record, K base, V base, step arguments)."""
+    geo, paged = geometry(kv, block_size, layout)
+    if geo.head_size not in HEAD_SIZES:
+        raise _lib.ShiftError(f"head_size {geo.head_size} is not one of {HEAD_SIZES}")
+    k_base, v_base = base_pointers(kv, geo)
+    if k_base % 16:
+        raise _lib.ShiftError("the cache must start on a 16-byte boundary")
+    ks, vs = scale_strides(k_scale, geo, "k_scale"), scale_strides(v_scale, geo, "v_scale")
+    stride, width = block_table_rows(block_tables)
+    reqs = block_tables.shape[0]
+    int32_vector(query_start, "query_start", reqs + 1)
+    int32_vector(seq_lens, "seq_lens", reqs)
+    cache = (paged, k_base, v_base, k_scale.data_ptr(), *ks, v_scale.data_ptr(), *vs)
+    step = (block_tables.data_ptr(), stride, width, query_start.data_ptr(), seq_lens.data_ptr(), reqs)
+    return geo, cache, step
+
+
+def append_block_scaled(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    kv: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,
+    query_start: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_size: int,
+    layout: str | None = None,
+    *,
+    check: bool = False,
+) -> None:
+    """Quantise the step's rows ``k``, ``v`` (``[tokens, heads, head_size]``, bf16, fp16 or fp32)
+    into the cache ``kv`` at their requests' last positions, in place.
+
+    A block's scale is the least power of two that brings its largest finite element to at
+    most 448 (at least 2^-64).  A block that already holds earlier tokens of its request
+    keeps them: its scale only grows, and their codes are requantised when it does
+    (exact but for codes that become subnormal).  A block whose first token is among the
+    rows starts afresh whatever its scale was.  Infinities become the largest code, NaN stays NaN.
+
+    Rows behind the last request are not written.  No two requests of a call may write the same block
+    (copy a shared block before appending to it).  Flagged and skipped: a block outside
+    the cache, positions past the block table, rows before position 0.
+    """
+    dev = cuda_on(None, kv=kv, k=k, v=v, k_scale=k_scale, v_scale=v_scale,
+                  block_tables=block_tables, query_start=query_start, seq_lens=seq_lens)
+    refuse_grad("append_block_scaled", "detach k and v", k, v)
+    geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
+                             layout)
+    code = dtype_code(k.dtype)
+    if code == _lib.E4M3 or v.dtype != k.dtype:
+        raise _lib.ShiftError(f"k and v must both be bf16, fp16 or fp32, got {k.dtype} and {v.dtype}")
+    rows = []
+    for name, t in (("k", k), ("v", v)):
+        rows += [t.data_ptr(), *heads_rows(t, name)]
+        if tuple(t.shape) != (k.shape[0], geo.heads, geo.head_size):
+            raise _lib.ShiftError(f"{name} must be [tokens, {geo.heads}, {geo.head_size}], got "
+                                  f"{tuple(t.shape)}")
+        vec = 16 // t.element_size()
+        if t.data_ptr() % 16 or t.stride(0) % vec or t.stride(1) % vec:
+            raise _lib.ShiftError(f"{name}'s rows must start on 16-byte boundaries")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride(), strict=True)):
+            raise _lib.ShiftError(f"{name} is written and must not repeat its elements")
+    if k_scale.data_ptr() == v_scale.data_ptr() and k_scale.numel():
+        raise _lib.ShiftError("k_scale and v_scale must be two tensors")
+    lib = _lib.load()
+    with Launch(dev) as on:
+        status = lib.mshift_append_block_scaled(code, *rows, k.shape[0], *cache, *step, on.err,
+                                                on.stream)
+    finish(status, "append_block_scaled", dev, check)
+
+
+def attend_block_scaled(
+    q: torch.Tensor,
+    kv: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,
+    query_start: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_size: int,
+    layout: str | None = None,
+    *,
+    max_query_len: int,
+    max_seq_len: int,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+    out: torch.Tensor | None = None,
+    return_lse: bool = False,
+    check: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of the step's rows ``q`` (``[tokens, query heads, head_size]``, bf16 or fp16) over the cache.
+
+    Query head ``j`` reads KV head ``j // (query heads / heads)``.  The row at position
+    ``p`` sees keys ``0..p`` of its request (``causal=False``: all of them), of those
+    only the last ``window`` (positions above ``p - window``) if ``window > 0``.  ``scale`` multiplies the
+    scores (default ``head_size ** -0.5``).  ``max_query_len`` and ``max_seq_len`` are host
+    bounds of the requests' row counts and ``seq_lens``; they size the launch, so a graph is captured with the
+    largest values its replays will meet.
+
+    Returns ``out`` (``q``'s type and shape), and with ``return_lse`` the rows' natural-log sums of
+    exponentials (fp32 ``[tokens, query heads]``).  A row that sees no key gets zeros and
+    ``-inf``.  Rows behind the last request are left as they were in a given ``out``, and
+    zeros (lse ``-inf``) otherwise.  Keys at positions that no row of a tile of rows may see are not
+    read, so stale codes there do no harm, NaN included; a NaN among the values of a token that later rows of the
+    same request see can reach its earlier rows too.  Value scales must be positive (below 2^-64 they are read
+    as 2^-64).
+
+    Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
+    the bounds (cut off there), positions past the block table (unseen).
+    """
+    dev = cuda_on(None, q=q, kv=kv, k_scale=k_scale, v_scale=v_scale, block_tables=block_tables,
+                  query_start=query_start, seq_lens=seq_lens, out=out)
+    refuse_grad("attend_block_scaled", "a cache of codes is not trained through", q, out)
+    geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
+                             layout)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.ShiftError(f"q must be bf16 or fp16, got {q.dtype}")
+    q_tok, q_head = heads_rows(q, "q")
+    rows, hq, head_size = q.shape
+    if head_size != geo.head_size or hq == 0 or hq % geo.heads:
+        raise _lib.ShiftError(f"q {tuple(q.shape)} does not fit {geo.heads} heads of {geo.head_size}")
+    if q.data_ptr() % 16 or q_tok % 8 or q_head % 8:
+        raise _lib.ShiftError("q's rows must start on 16-byte boundaries")
+    if not 0 <= max_query_len < 2**31 or not 0 <= max_seq_len < 2**31 or not 0 <= window < 2**31:
+        raise _lib.ShiftError("max_query_len, max_seq_len and window must be non-negative int32s")
+    scale = head_size ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise _lib.ShiftError(f"scale must be finite, got {scale}")
+    zero_tail = out is None
+    if out is not None:
+        heads_rows(out, "out", written=True)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise _lib.ShiftError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} "
+                                  f"{tuple(out.shape)}")
+        if out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8:
+            raise _lib.ShiftError("out's rows must start on 16-byte boundaries")
+        for name, t in (("q", q), ("kv", kv), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if overlap(out, t):
+                raise _lib.ShiftError(f"out shares memory with {name}")
+    lib = _lib.load()
+    code = dtype_code(q.dtype)
+    reqs = step[-1]
+    with Launch(dev) as on:
+        if out is None:
+            make = torch.zeros if reqs == 0 else torch.empty
+            out = make(q.shape, dtype=q.dtype, device=dev)
+        lse = None
+        if return_lse:
+            # rows behind the last request keep -inf where out keeps what it held
+            lse = (torch.empty if zero_tail and reqs else torch.full)(
+                (rows, hq), *(() if zero_tail and reqs else (-math.inf,)), dtype=torch.float32, device=dev)
+        need = lib.mshift_attend_workspace(rows, hq, geo.heads, head_size, reqs, max_query_len,
+                                           max_seq_len)
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        status = lib.mshift_attend_block_scaled(
+            code, q.data_ptr(), q_tok, q_head, rows, hq, *cache, *step, max_query_len, max_seq_len,
+            scale, int(causal), window, out.data_ptr(), out.stride(0), out.stride(1),
+            None if lse is None else lse.data_ptr(), int(zero_tail),
+            None if work is None else work.data_ptr(), max(need, 0), on.err, on.stream)
+    finish(status, "attend_block_scaled", dev, check)
+    return (out, lse) if return_lse else out

@@ -20,8 +20,18 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
-SOURCES = [PKG / "csrc" / "shift_kernels.cu"]
-HEADERS = [ROOT / "include" / "marathon_shift.h"]
+SOURCES = [
+    PKG / "csrc" / "shift_kernels.cu",
+    PKG / "csrc" / "block_maps.cu",
+    PKG / "csrc" / "rotary_axes.cu",
+    PKG / "csrc" / "append_block_scaled.cu",
+    PKG / "csrc" / "attend_block_scaled.cu",
+]
+HEADERS = [
+    ROOT / "include" / "marathon_shift.h",
+    PKG / "csrc" / "serve_common.cuh",
+    PKG / "csrc" / "attend.cuh",
+]
 LIB = PKG / "libmarathon_shift.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -40,6 +50,8 @@ def command(out: Path = LIB, extra: list[str] | None = None) -> list[str]:
         "-O3",
         "-lineinfo",
         "-std=c++17",
+        "--threads",
+        "0",  # the sources compile side by side
         "-Xcompiler",
         "-fPIC",
         "-Xcompiler",

@@ -1,0 +1,95 @@
+// attend.cuh — arguments and bookkeeping shared by the attention kernels over a
+// block-scaled cache (few rows: attend_block_scaled.cu, many: attend_rows.cu).
+//
+// Mathematics.  For a query row m at position x_m, keys j of its request:
+//     s_j = scale * ks[b(j), h] * (q_m . kcode_j)         natural-log score
+//     o   = sum_j e^{s_j} vs[b(j), h] vcode_j / sum_j e^{s_j}
+// The value scale is moved into the exponent: with t_j = s_j log2 e + log2 vs_j and
+// any reference M near max t_j,
+//     P_j = 2^(t_j - M),   acc = sum P_j vcode_j,   l = sum P_j / vs_j,   o = acc / l.
+// P_j is then in [0, 256] whatever the scales are and goes to f16 (11 bits) for the
+// matrix product without ever losing the row's largest term; l, acc and M are fp32.
+// One pass over the keys: M follows the maximum when it is passed by more than
+// 2^8 (f16 holds that), and acc and l are rescaled only then.
+//
+// e4m3 codes convert to f16 exactly.  A query row is brought to f16 by a power of two
+// that takes its largest element to [1, 2): a bf16 element keeps all its bits unless it is
+// below 2^-14 of that, and loses at most 2^-25 of the largest then.
+#pragma once
+
+#include "serve_common.cuh"
+
+namespace mshift {
+namespace serve {
+
+constexpr float kLazy = 8.0f;            // log2 of how far P may pass 1 before a rescale
+constexpr float kNoKey = -1e30f;         // M of a row that has seen no key
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttendArgs {
+  const void* q;
+  int64_t q_tok, q_head;  // elements
+  int rows;               // rows of q
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t blk, off, head;  // cache strides, bytes
+  int64_t num_blocks;
+  int bs;
+  const float* ks;
+  const float* vs;
+  int64_t ks_blk, ks_head, vs_blk, vs_head;
+  const int32_t* tables;
+  int64_t tab_stride;
+  int width;
+  const int32_t* qs;
+  const int32_t* lens;
+  int reqs, hq, hk, group;
+  int max_len;
+  float scale_log2;  // softmax scale * log2 e
+  int causal, window;
+  void* out;
+  int64_t o_tok, o_head;
+  float* lse;  // [rows, hq] or null
+  // keys are cut into splits of `chunk`; more than one: partial results
+  // part_o[row][head][split][D] and part_ml[row][head][split], joined afterwards
+  int chunk, nsplit;
+  float* part_o;
+  float2* part_ml;
+  int few_rows;  // requests of at most this many (token, group) rows go to the few-rows kernel
+  int zero_tail;
+  int max_q;     // the caller's bound on a request's tokens
+  uint32_t* err;
+};
+
+// One request's lengths, bounded by what the call's arrays hold.
+struct Request {
+  int q0, n, seq;
+  long long start;  // position of its first row
+};
+
+__device__ __forceinline__ Request request_of(const AttendArgs& a, int r, bool report) {
+  Request x;
+  x.q0 = row_start(a.qs, r, a.rows);
+  x.n = max(row_start(a.qs, r + 1, a.rows) - x.q0, 0);
+  const int len = a.lens[r];
+  x.start = (long long)len - x.n;
+  const long long held = (long long)a.width * a.bs;
+  x.seq = (int)min((long long)min(max(len, 0), a.max_len), held);
+  if (report) {
+    if (len > a.max_len || len < 0 || x.n > a.max_q || x.start < 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+    if (len > held) flag(a.err, MSHIFT_ERR_POOL);
+  }
+  return x;
+}
+
+// Keys [lo, hi) that the row at position x sees.
+__device__ __forceinline__ int2 seen(const AttendArgs& a, const Request& rq, long long x) {
+  const long long hi = a.causal ? min(x + 1, (long long)rq.seq) : rq.seq;
+  const long long lo = a.window > 0 ? max(x - a.window + 1, 0ll) : 0;
+  if (x < 0 || hi <= lo) return make_int2(0, 0);
+  return make_int2((int)lo, (int)hi);
+}
+
+}  // namespace serve
+}  // namespace mshift

@@ -1,0 +1,600 @@
+// attend_block_scaled.cu — attention over a block-scaled e4m3 paged cache: the kernel for
+// few query rows (decoding), the join of split results, and the entry point.
+//
+// A CTA has one (request, kv head, tile of NT * 8 query rows, split of the keys); its four
+// warps take 16-token steps in turn and join through shared memory at the end.
+// The rows are the request's (token, query head of the group) pairs, so the heads that
+// share a KV head read it once.
+//
+// Bound by HBM: 2 D bytes a (token, KV head) against 2 * 16 * D * 8 NT operations, so the
+// rows ride the narrow side of m16n8k16 and keys and values, as the wide side, go from
+// global memory to the matrix instructions through registers alone:
+//   scores  S^T[16 tokens x 8 rows] += K[16 x 16 dims] Q^T.  The order of the dims in a
+//           product is free, so lane (g, c) loads 16 contiguous codes of tokens g and g+8 at
+//           dims 64 u + 16 c, and Q is laid out to match once.
+//   values  O^T[16 dims x 8 rows] += V^T[16 dims x 16 tokens] P^T.  Lane (g, c) loads the
+//           codes of tokens 2c, 2c+1, 2c+8, 2c+9 at D/8 contiguous dims from g D/8; byte pairs of two
+//           tokens are the f16 pairs that the fragment wants.
+// P^T's fragment is S^T's transposed, which movmatrix does in registers.  The next step's codes are
+// loaded before this step's are used, so each warp keeps 16 tokens (4 KB at D = 128) in flight.
+#include "attend.cuh"
+
+namespace mshift {
+namespace serve {
+
+namespace {
+
+constexpr int kWarps = 4;
+
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// What a lane holds of one 16-token step.
+template <int D>
+struct Step {
+  static constexpr int kK = D / 64;                    // 16-byte loads of a K row
+  static constexpr int kV = D >= 128 ? D / 128 : 1;    // loads of a V row (8 bytes at D = 64)
+  uint4 k[2][kK];
+  uint4 v[4][kV];
+  float ks[2], vs[2];  // scales of tokens g and g + 8
+};
+
+template <int D, int NT, bool PAGE16, typename T>
+__global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArgs a, int tiles) {
+  constexpr int kRows = NT * 8;
+  constexpr int kMt = D / 16;  // 16-dim tiles of O^T
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ float s_o[kWarps][kRows][D + 4];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  if (a.zero_tail) {  // rows behind the last request
+    for (int64_t row = row_start(a.qs, a.reqs, a.rows) + (int64_t)blockIdx.x; row < a.rows;
+         row += gridDim.x) {
+      for (int i = threadIdx.x; i < a.hq * D; i += kWarps * 32)
+        static_cast<T*>(a.out)[row * a.o_tok + (i / D) * a.o_head + i % D] = Elem<T>::put(0.0f);
+      for (int i = threadIdx.x; i < a.hq && a.lse != nullptr; i += kWarps * 32)
+        a.lse[row * a.hq + i] = -INFINITY;
+    }
+  }
+  // heads fastest: in the NHD layouts neighbouring CTAs read neighbouring bytes
+  int64_t id = blockIdx.x;
+  const int h = (int)(id % a.hk);
+  id /= a.hk;
+  const int tile = (int)(id % tiles);
+  id /= tiles;
+  const int split = (int)(id % a.nsplit);
+  const int r = (int)(id / a.nsplit);
+  const Request rq = request_of(a, r, threadIdx.x == 0 && h == 0 && tile == 0 && split == 0);
+  const int all = rq.n * a.group, m0 = tile * kRows;
+  if (all > a.few_rows || m0 >= all) return;
+  const int live = min(kRows, all - m0);
+
+  // what this lane's rows 8 nt + 2c, 8 nt + 2c + 1 see, and the keys of the whole tile
+  int2 mine[NT][2];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int m = i * 8 + 2 * c + e;
+      mine[i][e] = m < live ? seen(a, rq, rq.start + (m0 + m) / a.group) : make_int2(0, 0);
+    }
+  const int2 head = seen(a, rq, max(rq.start + m0 / a.group, 0ll));
+  const int2 last = seen(a, rq, rq.start + (m0 + live - 1) / a.group);
+  // rows later in the tile see later keys at both ends
+  const int lo = max(head.x, split * a.chunk);
+  const int hi = min(last.y, split * a.chunk + a.chunk);
+  const int full_lo = max(last.x, lo);                       // keys that every row sees
+  const int full_hi = min(a.causal ? head.y : last.y, hi);
+  const bool all_live = rq.start + m0 / a.group >= 0;
+
+  // queries: f16 after a power of two for each row
+  uint32_t qf[NT][D / 16][2];
+  float rf[NT][2];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int m = i * 8 + g;
+    float x[D / 4];
+    float top = 0.0f;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {  // 8 elements of 16 bits
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (m < live) {
+          const T* src = static_cast<const T*>(a.q) + (rq.q0 + (m0 + m) / a.group) * a.q_tok +
+                         (h * a.group + (m0 + m) % a.group) * a.q_head + 64 * u + 16 * c + 8 * p;
+          w = *reinterpret_cast<const uint4*>(src);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Elem<T>::unpack(word(w, e), x + 16 * u + 8 * p + 2 * e);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(x[e]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // exponent of the largest element; rows of zeros, infinities or NaN as they are
+    int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+    if (e2 < -126 || e2 > 126) e2 = 0;
+    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const float* y = x + 16 * (s / 4) + 4 * (s % 4);
+      qf[i][s][0] = pack_f16x2(y[0] * down, y[1] * down);
+      qf[i][s][1] = pack_f16x2(y[2] * down, y[3] * down);
+    }
+    rf[i][0] = __shfl_sync(0xffffffffu, up, 8 * c);
+    rf[i][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+  }
+
+  float M[NT][2], l[NT][2], o[NT][kMt][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    M[i][0] = M[i][1] = kNoKey;
+    l[i][0] = l[i][1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+  }
+
+  const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
+  const uint8_t* kh = a.k + h * a.head;
+  const uint8_t* vh = a.v + h * a.head;
+  const float* ksh = a.ks + h * a.ks_head;
+  const float* vsh = a.vs + h * a.vs_head;
+  const int first = lo < hi ? lo / 16 : 0, steps = lo < hi ? (hi + 15) / 16 - first : 0;
+
+  // Loads step st's codes and scales; tokens outside [lo, hi) or in a bad block
+  // load nothing and count as zero codes, which their mask leaves out.  Returns
+  // the tokens (16 bits) whose block is good.
+  auto fetch = [&](int st, Step<D>& x) -> unsigned {
+    const int t0 = (first + st) * 16;
+    unsigned good;
+    long long base = 0;  // PAGE16: the step's place in its block; else that of token lane & 15
+    float ks = 0.0f, vs = 0.0f;
+    {
+      const int t = PAGE16 ? t0 : t0 + (lane & 15);
+      const int col = t / a.bs;
+      bool ok = PAGE16 || (t >= lo && t < hi);
+      if (ok) {
+        const int b = table[col];
+        ok = b >= 0 && b < a.num_blocks;
+        if (ok) {
+          base = b * a.blk + (t - col * a.bs) * a.off;
+          ks = ksh[b * a.ks_blk];
+          vs = vsh[b * a.vs_blk];
+        } else {
+          flag(a.err, MSHIFT_EBIT_SLOT);
+        }
+      }
+      if (PAGE16)
+        good = ok ? 0xffffu : 0u;
+      else
+        good = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+    }
+    unsigned in = good;  // tokens to load
+    if (t0 < lo) in &= 0xffffu << (lo - t0);
+    if (t0 + 16 > hi) in &= 0xffffu >> (t0 + 16 - hi);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = g + 8 * e;
+      const long long at = PAGE16 ? base + t * a.off : __shfl_sync(0xffffffffu, base, t);
+      x.ks[e] = PAGE16 ? ks : __shfl_sync(0xffffffffu, ks, t);
+      x.vs[e] = PAGE16 ? vs : __shfl_sync(0xffffffffu, vs, t);
+#pragma unroll
+      for (int u = 0; u < Step<D>::kK; ++u)
+        x.k[e][u] = (in >> t) & 1 ? load16(kh + at + 64 * u + 16 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = 2 * c + (e & 1) + 8 * (e >> 1);
+      const long long at = PAGE16 ? base + t * a.off : __shfl_sync(0xffffffffu, base, t);
+#pragma unroll
+      for (int u = 0; u < Step<D>::kV; ++u) {
+        x.v[e][u] = make_uint4(0, 0, 0, 0);
+        if ((in >> t) & 1) {
+          if constexpr (D == 64) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(vh + at + 8 * g));
+            x.v[e][u].x = w.x;
+            x.v[e][u].y = w.y;
+          } else {
+            x.v[e][u] = load16(vh + at + 128 * u + 16 * g);
+          }
+        }
+      }
+    }
+    return good;
+  };
+
+  Step<D> cur, nxt;
+  unsigned good = 0, good_nxt = 0;
+  if (warp < steps) good = fetch(warp, cur);
+  for (int st = warp; st < steps; st += kWarps) {
+    if (st + kWarps < steps) good_nxt = fetch(st + kWarps, nxt);
+    const int t0 = (first + st) * 16;
+
+    float s[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const uint32_t w0 = word(cur.k[0][d / 4], d % 4), w1 = word(cur.k[1][d / 4], d % 4);
+      const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)w0), e4m3x2_to_f16x2((uint16_t)w1),
+                             e4m3x2_to_f16x2((uint16_t)(w0 >> 16)),
+                             e4m3x2_to_f16x2((uint16_t)(w1 >> 16))};
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mma_f16(s[i], f, qf[i][d]);
+    }
+
+    // t = S ks rf + log2 vs, masked; a value scale of zero (or below 2^-64) reads as 2^-64
+    float vs[2], lv[2], rv[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      vs[e] = fmaxf(cur.vs[e], kScaleFloor);
+      lv[e] = __log2f(vs[e]);
+      rv[e] = __frcp_rn(vs[e]);
+    }
+    const bool whole = all_live && t0 >= full_lo && t0 + 16 <= full_hi && good == 0xffffu;
+    bool passed = false;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float t = fmaf(s[i][e] * rf[i][e & 1], cur.ks[e >> 1], lv[e >> 1]);
+        if (!whole) {
+          const int tok = g + 8 * (e >> 1), key = t0 + tok;
+          const int2 see = mine[i][e & 1];
+          if (!((good >> tok) & 1) || key < max(see.x, lo) || key >= min(see.y, hi)) t = -INFINITY;
+        }
+        s[i][e] = t;
+        passed |= t > M[i][e & 1] + kLazy;
+      }
+    if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(M[i][e], fmaxf(s[i][e], s[i][e + 2]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float by = ex2(M[i][e] - top);
+          M[i][e] = top;
+          l[i][e] *= by;
+#pragma unroll
+          for (int j = 0; j < kMt; ++j) {
+            o[i][j][e] *= by;
+            o[i][j][e + 2] *= by;
+          }
+        }
+    }
+    uint32_t p[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = ex2(s[i][e] - M[i][e & 1]);
+        l[i][e & 1] = fmaf(s[i][e], rv[e >> 1], l[i][e & 1]);
+      }
+      p[i][0] = transpose8x8(pack_f16x2(s[i][0], s[i][1]));
+      p[i][1] = transpose8x8(pack_f16x2(s[i][2], s[i][3]));
+    }
+    // two 16-bit pairs of a word: dims 2j (rows g) and 2j + 1 (rows g + 8) of tokens
+    // (2c, 2c+1) and (2c+8, 2c+9)
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) {
+      const int u = D == 64 ? 0 : j / 8, b = D == 64 ? j : j % 8;
+      const uint32_t sel = b % 2 == 0 ? 0x5140 : 0x7362;
+      const uint32_t x = __byte_perm(word(cur.v[0][u], b / 2), word(cur.v[1][u], b / 2), sel);
+      const uint32_t y = __byte_perm(word(cur.v[2][u], b / 2), word(cur.v[3][u], b / 2), sel);
+      const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)x), e4m3x2_to_f16x2((uint16_t)(x >> 16)),
+                             e4m3x2_to_f16x2((uint16_t)y), e4m3x2_to_f16x2((uint16_t)(y >> 16))};
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mma_f16(o[i][j], f, p[i]);
+    }
+    cur = nxt;
+    good = good_nxt;
+  }
+
+  // join the warps
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[i][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      const int m = i * 8 + 2 * c + e;
+      if (g == 0) {
+        s_m[warp][m] = M[i][e];
+        s_l[warp][m] = x;
+      }
+#pragma unroll
+      for (int j = 0; j < kMt; ++j) {
+        const int dim = D == 64 ? 8 * g + 2 * j : 128 * (j / 8) + 16 * g + 2 * (j % 8);
+        *reinterpret_cast<float2*>(&s_o[warp][m][dim]) = make_float2(o[i][j][e], o[i][j][e + 2]);
+      }
+    }
+  __syncthreads();
+  for (int at = threadIdx.x; at < live * (D / 4); at += kWarps * 32) {
+    const int m = at / (D / 4), d = at % (D / 4) * 4;
+    float top = s_m[0][m];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][m]);
+    float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float by = ex2(s_m[w][m] - top);
+      sum = fmaf(s_l[w][m], by, sum);
+      const float4 y = *reinterpret_cast<const float4*>(&s_o[w][m][d]);
+      x[0] = fmaf(y.x, by, x[0]);
+      x[1] = fmaf(y.y, by, x[1]);
+      x[2] = fmaf(y.z, by, x[2]);
+      x[3] = fmaf(y.w, by, x[3]);
+    }
+    const int64_t row = rq.q0 + (m0 + m) / a.group;
+    const int hq = h * a.group + (m0 + m) % a.group;
+    if (a.nsplit > 1) {
+      const int64_t part = (row * a.hq + hq) * a.nsplit + split;
+      *reinterpret_cast<float4*>(a.part_o + part * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      if (d == 0) a.part_ml[part] = make_float2(top, sum);
+    } else {
+      const bool any = top > kNoKey;
+      const float by = any ? 1.0f / sum : 0.0f;
+      T* dst = static_cast<T*>(a.out) + row * a.o_tok + hq * a.o_head + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[e] = Elem<T>::put(any ? x[e] * by : 0.0f);
+      if (d == 0 && a.lse != nullptr)
+        a.lse[row * a.hq + hq] = any ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    }
+  }
+}
+
+// o = sum_s 2^(M_s - M) acc_s / sum_s 2^(M_s - M) l_s over the splits of one (row, head);
+// a CTA for each, a thread for each dim.
+template <int D, typename T>
+__global__ void __launch_bounds__(D) attend_join_kernel(const AttendArgs a) {
+  extern __shared__ float s_by[];
+  __shared__ float s_red[2][D / 32];
+  const int64_t row = blockIdx.x / a.hq;
+  const int hq = blockIdx.x % a.hq, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= row_start(a.qs, a.reqs, a.rows)) return;
+  const int r = find_request(a.reqs, row, [&](int i) { return (long long)row_start(a.qs, i, a.rows); });
+  const Request rq = request_of(a, r, false);
+  if (row < rq.q0 || row >= rq.q0 + rq.n) return;
+  const int2 see = seen(a, rq, rq.start + (row - rq.q0));
+  // splits that hold a key of this row; at least one, for a row without keys
+  const int s0 = see.x / a.chunk, s1 = max((see.y + a.chunk - 1) / a.chunk, s0 + 1);
+  const int64_t part = blockIdx.x * (int64_t)a.nsplit;
+  float top = kNoKey;
+  for (int s = s0 + tid; s < s1; s += D) top = fmaxf(top, a.part_ml[part + s].x);
+  for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) s_red[0][warp] = top;
+  __syncthreads();
+  for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[0][w]);
+  float sum = 0.0f;
+  for (int s = s0 + tid; s < s1; s += D) {
+    const float2 ml = a.part_ml[part + s];
+    const float by = ex2(ml.x - top);
+    s_by[s - s0] = by;
+    sum = fmaf(ml.y, by, sum);
+  }
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) s_red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int w = 0; w < D / 32; ++w) sum += s_red[1][w];
+  float x = 0.0f;
+  const float* src = a.part_o + (part + s0) * D + tid;
+#pragma unroll 8
+  for (int s = 0; s < s1 - s0; ++s) x = fmaf(src[(int64_t)s * D], s_by[s], x);
+  const bool any = top > kNoKey;
+  static_cast<T*>(a.out)[row * a.o_tok + hq * a.o_head + tid] = Elem<T>::put(any ? x / sum : 0.0f);
+  if (tid == 0 && a.lse != nullptr)
+    a.lse[row * a.hq + hq] = any ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+template <int D, int NT, typename T>
+cudaError_t launch_few(const AttendArgs& a, int64_t most_rows, cudaStream_t stream) {
+  const int tiles = (int)((most_rows + NT * 8 - 1) / (NT * 8));
+  const int64_t grid = (int64_t)a.reqs * a.nsplit * tiles * a.hk;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  // whole 16-token steps inside one block need one table entry; other block
+  // sizes look each token up
+  if (a.bs % 16 == 0)
+    attend_few_kernel<D, NT, true, T><<<(unsigned)grid, kWarps * 32, 0, stream>>>(a, tiles);
+  else
+    attend_few_kernel<D, NT, false, T><<<(unsigned)grid, kWarps * 32, 0, stream>>>(a, tiles);
+  return cudaGetLastError();
+}
+
+template <int D, typename T>
+cudaError_t launch_join(const AttendArgs& a, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)a.rows * a.hq));
+  cfg.blockDim = dim3(D);
+  cfg.dynamicSmemBytes = sizeof(float) * a.nsplit;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T>, a);
+}
+
+template <int D, typename T>
+cudaError_t launch_all(const AttendArgs& a, int64_t most_rows, cudaStream_t stream) {
+  // 8 rows a tile, or 16 where a request has more: twice the rows for the same codes
+  cudaError_t e;
+  if constexpr (D == 256) {
+    e = launch_few<D, 1, T>(a, most_rows, stream);
+  } else {
+    e = most_rows <= 8 ? launch_few<D, 1, T>(a, most_rows, stream)
+                       : launch_few<D, 2, T>(a, most_rows, stream);
+  }
+  if (e == cudaSuccess && a.nsplit > 1) e = launch_join<D, T>(a, stream);
+  return e;
+}
+
+template <typename T>
+int attend_dispatch(const AttendArgs& a, int head_size, cudaStream_t stream) {
+  const int64_t most_rows = min((int64_t)min(a.max_q, a.rows) * a.group, (int64_t)a.few_rows);
+  cudaError_t e;
+  switch (head_size) {
+    case 64: e = launch_all<64, T>(a, most_rows, stream); break;
+    case 128: e = launch_all<128, T>(a, most_rows, stream); break;
+    case 256: e = launch_all<256, T>(a, most_rows, stream); break;
+    default: return MSHIFT_EUNSUPPORTED;
+  }
+  return e == cudaSuccess ? MSHIFT_OK : cuda_fail(e);
+}
+
+constexpr int kMaxSplits = 1024;
+
+// Tokens of a split.  Enough splits that the CTAs of all requests, heads and tiles fill
+// the GPU's 148 SMs a few times over, but no split so short that its start-up shows.
+int chunk_for(int64_t units, int max_len) {
+  const int64_t want = 148 * 8;
+  int64_t splits = (want + units - 1) / units;
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  int64_t chunk = ((int64_t)max_len + splits - 1) / splits;
+  chunk = chunk < 256 ? 256 : chunk > 2048 ? 2048 : chunk;
+  const int64_t least = ((int64_t)max_len + kMaxSplits - 1) / kMaxSplits;
+  if (chunk < least) chunk = least;
+  return (int)((chunk + 63) / 64 * 64);
+}
+
+void plan(int32_t rows, int32_t hq, int32_t hk, int32_t reqs, int32_t max_q, int32_t max_len,
+          int* chunk, int* nsplit) {
+  const int64_t most = (int64_t)(max_q < rows ? max_q : rows) * (hq / hk);
+  const int64_t tiles = most <= 8 ? 1 : (most + 15) / 16;
+  *chunk = chunk_for((int64_t)reqs * hk * tiles, max_len);
+  *nsplit = max_len > 0 ? (max_len + *chunk - 1) / *chunk : 1;
+}
+
+}  // namespace
+}  // namespace serve
+}  // namespace mshift
+
+extern "C" {
+
+int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk, int32_t head_size,
+                                int32_t reqs, int32_t max_query_len, int32_t max_seq_len) {
+  if (rows < 0 || hq <= 0 || hk <= 0 || hq % hk != 0 || head_size <= 0 || reqs < 0 ||
+      max_query_len < 0 || max_seq_len < 0)
+    return -1;
+  if (rows == 0 || reqs == 0) return 0;
+  int chunk, nsplit;
+  mshift::serve::plan(rows, hq, hk, reqs, max_query_len, max_seq_len, &chunk, &nsplit);
+  return nsplit > 1 ? (int64_t)rows * hq * nsplit * (head_size + 2) * 4 : 0;
+}
+
+int mshift_attend_block_scaled(
+    int32_t dtype, const void* q, int64_t q_tok, int64_t q_head, int32_t rows, int32_t hq,
+    const mshift_paged* paged, const void* k_base, const void* v_base, const float* k_scale,
+    int64_t ks_blk, int64_t ks_head, const float* v_scale, int64_t vs_blk, int64_t vs_head,
+    const int32_t* block_tables, int64_t table_stride, int32_t width, const int32_t* query_start,
+    const int32_t* seq_lens, int32_t reqs, int32_t max_query_len, int32_t max_seq_len, float scale,
+    int32_t causal, int32_t window, void* out, int64_t o_tok, int64_t o_head, float* lse,
+    int32_t zero_tail, void* workspace, int64_t workspace_bytes, uint32_t* err, void* stream) {
+  using namespace mshift;
+  using namespace mshift::serve;
+  if (paged == nullptr || rows < 0 || reqs < 0 || hq <= 0 || width < 0 || table_stride < width ||
+      max_query_len < 0 || max_seq_len < 0 || window < 0)
+    return MSHIFT_EINVAL;
+  if (paged->dtype != MSHIFT_E4M3 || (dtype != MSHIFT_BF16 && dtype != MSHIFT_F16))
+    return MSHIFT_EUNSUPPORTED;
+  if (paged->heads <= 0 || hq % paged->heads != 0 || paged->block_size <= 0 ||
+      paged->num_blocks < 0)
+    return MSHIFT_EINVAL;
+  if (rows == 0 || reqs == 0) return MSHIFT_OK;
+  if (q == nullptr || k_base == nullptr || v_base == nullptr || k_scale == nullptr ||
+      v_scale == nullptr || (width > 0 && block_tables == nullptr) || query_start == nullptr ||
+      seq_lens == nullptr || out == nullptr || err == nullptr)
+    return MSHIFT_EINVAL;
+  const auto odd = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+  if (odd(q) || odd(k_base) || odd(v_base) || q_tok % 8 || q_head % 8 || paged->blk_stride % 16 ||
+      paged->off_stride % 16 || paged->head_stride % 16)
+    return MSHIFT_EINVAL;
+  int chunk, nsplit;
+  plan(rows, hq, paged->heads, reqs, max_query_len, max_seq_len, &chunk, &nsplit);
+  const int64_t parts = (int64_t)rows * hq * nsplit;
+  if (nsplit > 1 && (workspace == nullptr || odd(workspace) ||
+                     workspace_bytes < parts * (paged->head_size + 2) * 4))
+    return MSHIFT_EINVAL;
+  AttendArgs a{};
+  a.q = q;
+  a.q_tok = q_tok;
+  a.q_head = q_head;
+  a.rows = rows;
+  a.k = static_cast<const uint8_t*>(k_base);
+  a.v = static_cast<const uint8_t*>(v_base);
+  a.blk = paged->blk_stride;
+  a.off = paged->off_stride;
+  a.head = paged->head_stride;
+  a.num_blocks = paged->num_blocks;
+  a.bs = paged->block_size;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.ks_blk = ks_blk;
+  a.ks_head = ks_head;
+  a.vs_blk = vs_blk;
+  a.vs_head = vs_head;
+  a.tables = block_tables;
+  a.tab_stride = table_stride;
+  a.width = width;
+  a.qs = query_start;
+  a.lens = seq_lens;
+  a.reqs = reqs;
+  a.hq = hq;
+  a.hk = paged->heads;
+  a.group = hq / paged->heads;
+  a.max_len = max_seq_len;
+  a.scale_log2 = scale * kLog2e;
+  a.causal = causal;
+  a.window = window;
+  a.out = out;
+  a.o_tok = o_tok;
+  a.o_head = o_head;
+  a.lse = lse;
+  a.chunk = chunk;
+  a.nsplit = nsplit;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + parts * paged->head_size);
+  a.few_rows = INT32_MAX;
+  a.zero_tail = zero_tail;
+  a.max_q = max_query_len;
+  a.err = err;
+  auto s = static_cast<cudaStream_t>(stream);
+  return dtype == MSHIFT_BF16 ? attend_dispatch<__nv_bfloat16>(a, paged->head_size, s)
+                              : attend_dispatch<__half>(a, paged->head_size, s);
+}
+
+}  // extern "C"

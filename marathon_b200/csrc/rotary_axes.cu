@@ -1,0 +1,185 @@
+// rotary_axes.cu — rotary positions with several axes, queries and keys in one launch.
+//
+// Frequency i of a token turns by a = positions[axes[i]][token] * inv_freq[i]:
+//     out[i]        = x[i] * cos a - x[i + half] * sin a
+//     out[i + half] = x[i + half] * cos a + x[i] * sin a
+// (NeoX half-split pairs; sin changes sign for the inverse).  The path is bound by
+// HBM: each element is read once and written once, in 16-byte vectors that are
+// rotary partners, so a thread holds both halves of its pairs.
+//
+// The angle.  A far position times an fp32 frequency has an fp32 rounding of up
+// to 0.06 rad at a million, so the angle is formed in turns, modulo one, in 64-bit
+// fixed point: F = inv_freq / 2pi as a fraction of 2^64 (from fp64, 53 bits), and
+// position * F wraps modulo 2^64, which is modulo one turn.  What is left, in
+// [-1/2, 1/2) turns, goes to fp32 sincospi.  The angle's error is below
+// position * 2^-53 + 2^-24 turns.  One sin and cos a (token, frequency), shared by all heads
+// through shared memory.
+#include <type_traits>
+
+#include "serve_common.cuh"
+
+namespace mshift {
+namespace serve {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 4;      // most tokens of a CTA
+constexpr int kRotMaxHalf = 256;   // frequencies: rotary up to 512
+
+struct RotArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_tok, q_head, k_tok, k_head, qo_tok, qo_head, ko_tok, ko_head;  // elements
+  int64_t n;
+  int hq, hk, head_size, half;
+  const void* positions;
+  int64_t pos_axis;  // elements between axes
+  int pos64, n_axes;
+  const float* inv_freq;
+  const int32_t* axes;
+  float sign;
+  int tokens, slices;  // tokens a CTA, head slices
+  uint32_t* err;
+};
+
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Pack {
+  T x[VEC];
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRotThreads) rotary_axes_kernel(const RotArgs a) {
+  __shared__ float2 s_cs[kRotTokens * kRotMaxHalf];
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int here = (int)min((int64_t)a.tokens, a.n - t0);
+  for (int u = threadIdx.x; u < here * a.half; u += kRotThreads) {
+    const int tok = u / a.half, i = u - tok * a.half;
+    int axis = a.axes != nullptr ? a.axes[i] : 0;
+    if (axis < 0 || axis >= a.n_axes) {
+      flag(a.err, MSHIFT_EBIT_TABLE);
+      axis = 0;
+    }
+    const int64_t at = axis * a.pos_axis + t0 + tok;
+    const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
+                                : static_cast<const int32_t*>(a.positions)[at];
+    double f = (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / 2pi
+    f -= floor(f);
+    const uint64_t turns = (uint64_t)pos * __double2ull_rn(f * 0x1p64);
+    float sn, cs;
+    sincospif((float)(int64_t)turns * 0x1p-63f, &sn, &cs);
+    s_cs[u] = make_float2(cs, sn * a.sign);
+  }
+  __syncthreads();
+
+  using P = Pack<T, VEC>;
+  using E = Elem<T>;
+  const int rot = a.half / VEC;  // vectors of pairs in a head
+  // the tail past the rotary is copied where the result goes elsewhere
+  const int tail = (a.head_size - 2 * a.half) / VEC;
+  const int per = rot + tail;
+  const int heads = a.hq + a.hk;
+  for (int u = threadIdx.x; u < here * per * a.slices; u += kRotThreads) {
+    const int j = u % per, rest = u / per;
+    const int tok = rest % here, slice = rest / here;
+    const int64_t t = t0 + tok;
+    float2 cs[VEC];
+    if (j < rot) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) cs[e] = s_cs[tok * a.half + j * VEC + e];
+    }
+#pragma unroll 2
+    for (int h = slice; h < heads; h += a.slices) {
+      const T* src;
+      T* dst;
+      if (h < a.hq) {
+        src = static_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head;
+        dst = static_cast<T*>(a.q_out) + t * a.qo_tok + h * a.qo_head;
+      } else {
+        src = static_cast<const T*>(a.k) + t * a.k_tok + (h - a.hq) * a.k_head;
+        dst = static_cast<T*>(a.k_out) + t * a.ko_tok + (h - a.hq) * a.ko_head;
+      }
+      if (j >= rot) {
+        const int at = 2 * a.half + (j - rot) * VEC;
+        if (dst != src) *reinterpret_cast<P*>(dst + at) = *reinterpret_cast<const P*>(src + at);
+        continue;
+      }
+      const P x = *reinterpret_cast<const P*>(src + j * VEC);
+      const P y = *reinterpret_cast<const P*>(src + a.half + j * VEC);
+      P xo, yo;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xf = E::get(x.x[e]), yf = E::get(y.x[e]);
+        xo.x[e] = E::put(xf * cs[e].x - yf * cs[e].y);
+        yo.x[e] = E::put(yf * cs[e].x + xf * cs[e].y);
+      }
+      *reinterpret_cast<P*>(dst + j * VEC) = xo;
+      *reinterpret_cast<P*>(dst + a.half + j * VEC) = yo;
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_rotary(RotArgs a, cudaStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  auto whole = [](const void* p, int64_t tok, int64_t head) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % kVec == 0 &&
+                            head % kVec == 0);
+  };
+  // 16-byte vectors where every row starts on one and the halves split into
+  // whole vectors; element by element otherwise (odd strides or frequencies)
+  const bool vec = whole(a.q, a.q_tok, a.q_head) && whole(a.k, a.k_tok, a.k_head) &&
+                   whole(a.q_out, a.qo_tok, a.qo_head) && whole(a.k_out, a.ko_tok, a.ko_head) &&
+                   a.half % kVec == 0 && a.head_size % kVec == 0;
+  // one token a CTA until that fills the GPU several times over, then four, which
+  // share the CTA's start-up
+  a.tokens = a.n >= 4096 ? kRotTokens : 1;
+  const int v = vec ? kVec : 1;
+  const int per = a.half / v + (a.head_size - 2 * a.half) / v;
+  a.slices = max(1, min(a.hq + a.hk, kRotThreads / (a.tokens * max(per, 1))));
+  const int64_t grid = (a.n + a.tokens - 1) / a.tokens;
+  if (vec)
+    rotary_axes_kernel<T, kVec><<<(unsigned)grid, kRotThreads, 0, stream>>>(a);
+  else
+    rotary_axes_kernel<T, 1><<<(unsigned)grid, kRotThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace serve
+}  // namespace mshift
+
+extern "C" int mshift_rotary_axes(int32_t dtype, const void* q, int64_t q_tok, int64_t q_head,
+                                  void* q_out, int64_t qo_tok, int64_t qo_head, int32_t hq,
+                                  const void* k, int64_t k_tok, int64_t k_head, void* k_out,
+                                  int64_t ko_tok, int64_t ko_head, int32_t hk, int64_t n,
+                                  int32_t head_size, int32_t rotary, const void* positions,
+                                  int64_t pos_axis_stride, int32_t pos_is_64, int32_t n_axes,
+                                  const float* inv_freq, const int32_t* axes, int32_t inverse,
+                                  uint32_t* err, void* stream) {
+  using namespace mshift;
+  using namespace mshift::serve;
+  if (n < 0 || n > INT32_MAX || hq < 0 || hk < 0 || head_size <= 0 || rotary < 0 ||
+      rotary % 2 != 0 || rotary > head_size || n_axes <= 0 || head_size > 1024)
+    return MSHIFT_EINVAL;
+  if (rotary > 2 * kRotMaxHalf) return MSHIFT_EUNSUPPORTED;
+  if (n == 0 || hq + hk == 0) return MSHIFT_OK;
+  if ((hq > 0 && (q == nullptr || q_out == nullptr)) ||
+      (hk > 0 && (k == nullptr || k_out == nullptr)) || positions == nullptr || err == nullptr ||
+      (rotary > 0 && inv_freq == nullptr))
+    return MSHIFT_EINVAL;
+  const RotArgs a{hq ? q : nullptr, hk ? k : nullptr, hq ? q_out : nullptr, hk ? k_out : nullptr,
+                  q_tok, q_head, k_tok, k_head, qo_tok, qo_head, ko_tok, ko_head, n, hq, hk,
+                  head_size, rotary / 2, positions, pos_axis_stride, pos_is_64, n_axes, inv_freq,
+                  axes, inverse ? -1.0f : 1.0f, 1, 1, err};
+  auto s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  switch (dtype) {
+    case MSHIFT_BF16: e = launch_rotary<__nv_bfloat16>(a, s); break;
+    case MSHIFT_F16: e = launch_rotary<__half>(a, s); break;
+    case MSHIFT_F32: e = launch_rotary<float>(a, s); break;
+    default: return MSHIFT_EUNSUPPORTED;
+  }
+  return e == cudaSuccess ? MSHIFT_OK : cuda_fail(e);
+}

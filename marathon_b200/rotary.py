@@ -1,0 +1,142 @@
+"""Rotary positions with several axes (time, height, width), queries and keys in one launch.
+
+The shift path rotates by one axis: a delta for each segment
+(:func:`marathon_b200.shift_kernels.rope_tables`).  Models that see images or
+video give a token one position for each axis, and each rotary frequency takes
+its angle from one of them.  :func:`rotary_axes` applies that to queries and keys; with deltas in the place of
+positions it re-rotates reused keys (R(p + d) = R(d) R(p) holds axis by axis),
+and ``inverse`` undoes it, which is also its transpose: the gradient of the result
+goes back to the inputs through ``inverse=True``.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Sequence
+
+import torch
+
+from . import _lib
+from ._serve import Launch, cuda_on, finish, heads_rows, int32_vector, overlap, refuse_grad
+from .paged import dtype_code
+
+__all__ = ["axis_map", "rotary_axes"]
+
+
+def axis_map(sections: Sequence[int], interleaved: bool = False, device=None) -> torch.Tensor:
+    """The axis of each rotary frequency (int32), from how many frequencies each axis has.
+
+    Contiguous: ``sections[0]`` frequencies of axis 0, then axis 1, and so on.
+    ``interleaved``: frequency ``i`` belongs to axis ``i % len(sections)`` as long as that
+    axis has frequencies left in its turn (``i < sections[axis] * len(sections)``), and to axis 0 otherwise.
+    """
+    n, half = len(sections), sum(sections)
+    if n == 0 or min(sections) < 0:
+        raise _lib.ShiftError(f"sections must be counts of frequencies, got {tuple(sections)}")
+    if interleaved:
+        axes = [i % n if i < sections[i % n] * n else 0 for i in range(half)]
+        if any(axes.count(a) != sections[a] for a in range(n)):
+            raise _lib.ShiftError(f"sections {tuple(sections)} cannot be interleaved: an axis behind "
+                                  "the first has more frequencies than turns")
+    else:
+        axes = [a for a, m in enumerate(sections) for _ in range(m)]
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def rotary_axes(
+    q: torch.Tensor | None,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    axes: torch.Tensor | None = None,
+    *,
+    inverse: bool = False,
+    inplace: bool = False,
+    check: bool = False,
+) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """``q`` and ``k`` (``[tokens, heads, head_size]``, either may be None) rotated by their positions.
+
+    ``positions`` is int32 or int64, ``[tokens]`` or ``[n_axes, tokens]``, of any
+    sign; ``inv_freq`` fp32 ``[rotary / 2]`` with ``rotary <= head_size`` (the tail
+    passes through); ``axes`` int32 ``[rotary / 2]`` (:func:`axis_map`), or None where all
+    frequencies take axis 0.  NeoX half-split pairs, bf16, fp16 or fp32, rotated in fp32 and
+    rounded once.  Angles are exact modulo a turn to fp32 precision at any position.  Any
+    token and head strides; ``inplace`` writes into ``q`` and ``k`` themselves.  All tensors on one
+    GPU.  An entry of ``axes`` that names no axis is flagged.
+    """
+    one = q if q is not None else k
+    if one is None:
+        raise _lib.ShiftError("rotary_axes needs q or k")
+    dev = cuda_on(None, q=q, k=k, positions=positions, inv_freq=inv_freq, axes=axes)
+    refuse_grad("rotary_axes", "its gradient is rotary_axes(..., inverse=True) of the result's", q, k)
+    code = dtype_code(one.dtype)
+    if code == _lib.E4M3:
+        raise _lib.ShiftError("rotary_axes takes bf16, fp16 or fp32")
+    if one.dim() != 3:
+        raise _lib.ShiftError(f"q and k must be [tokens, heads, head_size], got {tuple(one.shape)}")
+    n, _, head_size = one.shape
+    if q is not None and k is not None and (k.dtype != q.dtype or k.dim() != 3
+                                            or k.shape[0] != n or k.shape[2] != head_size):
+        raise _lib.ShiftError(f"q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} differ in "
+                              "type, tokens or head size")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise _lib.ShiftError("inv_freq must be an fp32 vector")
+    half = inv_freq.numel()
+    if 2 * half > head_size:
+        raise _lib.ShiftError(f"rotary {2 * half} > head_size {head_size}")
+    if half > 256 or head_size > 1024:
+        raise _lib.ShiftError("rotary_axes takes head sizes up to 1024 and rotary up to 512")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
+            or positions.shape[-1] != n:
+        raise _lib.ShiftError(f"positions must be int32 or int64 [{n}] or [axes, {n}], got "
+                              f"{positions.dtype} {tuple(positions.shape)}")
+    n_axes = positions.shape[0] if positions.dim() == 2 else 1
+    if n_axes == 0:
+        raise _lib.ShiftError("positions have no axis")
+    if axes is not None:
+        int32_vector(axes, "axes", half)
+    elif n_axes > 1:
+        raise _lib.ShiftError(f"positions have {n_axes} axes: axes must say which each frequency takes")
+    if n > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    if half > 1 and inv_freq.stride(0) != 1:
+        inv_freq = inv_freq.contiguous()
+    ins, outs = [], []
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            ins += [None, 0, 0]
+            continue
+        ins += [t.data_ptr(), *heads_rows(t, name, inplace)]
+    if inplace and q is not None and k is not None and overlap(q, k) and _interleaved_clash(q, k):
+        raise _lib.ShiftError("q and k share elements and cannot both be rotated in place")
+    if inplace:
+        for t in (positions, inv_freq, axes):
+            if t is not None and any(x is not None and overlap(t, x) for x in (q, k)):
+                raise _lib.ShiftError("an argument shares memory with a tensor rotated in place")
+    lib = _lib.load()
+    with Launch(dev) as on:
+        got = []
+        for t in (q, k):
+            o = t if t is None or inplace else torch.empty(t.shape, dtype=t.dtype, device=dev)
+            got.append(o)
+            outs += [None, 0, 0] if o is None else [o.data_ptr(), o.stride(0), o.stride(1)]
+        status = lib.mshift_rotary_axes(
+            code, *ins[:3], *outs[:3], 0 if q is None else q.shape[1], *ins[3:], *outs[3:],
+            0 if k is None else k.shape[1], n, head_size, 2 * half, positions.data_ptr(),
+            positions.stride(0) if n_axes > 1 else n, int(positions.dtype == torch.int64), n_axes,
+            inv_freq.data_ptr(), None if axes is None else axes.data_ptr(), int(inverse), on.err,
+            on.stream)
+    finish(status, "rotary_axes", dev, check)
+    return got[0], got[1]
+
+
+def _interleaved_clash(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether overlapping address ranges share elements.  Views of one fused projection
+    ([tokens, (q heads + k heads) * head_size]) interleave by token without sharing any."""
+    if q.stride(0) != k.stride(0) or q.shape[0] < 2:
+        return True
+    row = q.stride(0)
+    width_q = (q.shape[1] - 1) * q.stride(1) + q.shape[2]
+    width_k = (k.shape[1] - 1) * k.stride(1) + k.shape[2]
+    gap = (k.data_ptr() - q.data_ptr()) // q.element_size()
+    return not (0 <= gap - width_q and gap + width_k <= row) and \
+        not (0 <= -gap - width_k and -gap + width_q <= row)

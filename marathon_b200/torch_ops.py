@@ -19,6 +19,12 @@ raise.
   layout)`` -- paged rows back into the store rows at the same positions
   (``vllm_shift_connector.py:539-553``), all layers in one launch.
 
+* ``marathon::block_maps``, ``marathon::rotary_axes``, ``marathon::append_block_scaled`` and
+  ``marathon::attend_block_scaled`` -- the serving operators over a block-scaled e4m3 cache,
+  with the arguments of :mod:`marathon_b200.block_maps`, :mod:`~marathon_b200.rotary` and
+  :mod:`~marathon_b200.block_scaled`.  ``rotary_axes`` records gradients of ``q`` and ``k``
+  (the rotation by the negative angles).
+
 ``stores`` is flat, session-major: session ``s``'s layer ``l`` buffer is
 ``stores[s * n_layers + l]`` (``[capacity, heads, 2*head_size]``).
 ``segments`` is an int64 ``[n, 5]`` tensor of ``(session, src_start,
@@ -33,7 +39,10 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from .block_maps import block_maps
+from .block_scaled import append_block_scaled, attend_block_scaled
 from .paged import KVLayers
+from .rotary import rotary_axes
 from .shift_kernels import Launcher, RopeShift, RunSpec, ShiftError, StoreView, scatter_shifted
 
 _launchers: dict = {}
@@ -137,3 +146,82 @@ def _(stores, kv, segments, block_tables, inv_freq, block_size, layout, k_scales
 @_shift_save_op.register_fake
 def _(kv, stores, segments, block_tables, block_size, layout) -> None:
     return None
+
+
+# ------------------------------------------------------------ serving operators
+@torch.library.custom_op("marathon::block_maps", mutates_args=("block_tables",))
+def _block_maps_op(
+    cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
+    free_blocks: torch.Tensor, free_head: torch.Tensor, block_size: int, tokens: int,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    m = block_maps(cached_lens, new_lens, block_tables, free_blocks, free_head, block_size, tokens)
+    return m.query_start, m.seq_lens, m.slots, m.positions, m.free_head
+
+
+@_block_maps_op.register_fake
+def _(cached_lens, new_lens, block_tables, free_blocks, free_head, block_size, tokens):
+    reqs = cached_lens.shape[0]
+    rows = [cached_lens.new_empty(tokens, dtype=torch.int64) for _ in range(2)]
+    return (cached_lens.new_empty(reqs + 1), cached_lens.new_empty(reqs), *rows,
+            cached_lens.new_empty(1))
+
+
+@torch.library.custom_op("marathon::rotary_axes", mutates_args=())
+def _rotary_axes_op(
+    q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+    axes: torch.Tensor | None = None, inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    # detached: gradients are recorded around the operator, not in it
+    return rotary_axes(q.detach(), k.detach(), positions, inv_freq, axes, inverse=inverse)
+
+
+@_rotary_axes_op.register_fake
+def _(q, k, positions, inv_freq, axes=None, inverse=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def _rotary_axes_setup(ctx, inputs, output) -> None:
+    _, _, *ctx.tables, ctx.inverse = inputs
+
+
+def _rotary_axes_backward(ctx, dq, dk):
+    # a sum's gradient comes as one element read many times: the kernel wants contiguous heads
+    dq, dk = (d if d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
+    return *torch.ops.marathon.rotary_axes(dq, dk, *ctx.tables, not ctx.inverse), None, None, None, None
+
+
+_rotary_axes_op.register_autograd(_rotary_axes_backward, setup_context=_rotary_axes_setup)
+
+
+@torch.library.custom_op("marathon::append_block_scaled", mutates_args=("kv", "k_scale", "v_scale"))
+def _append_block_scaled_op(
+    k: torch.Tensor, v: torch.Tensor, kv: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    block_tables: torch.Tensor, query_start: torch.Tensor, seq_lens: torch.Tensor, block_size: int,
+    layout: str,
+) -> None:
+    append_block_scaled(k, v, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
+                        layout)
+
+
+@_append_block_scaled_op.register_fake
+def _(k, v, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size, layout) -> None:
+    return None
+
+
+@torch.library.custom_op("marathon::attend_block_scaled", mutates_args=())
+def _attend_block_scaled_op(
+    q: torch.Tensor, kv: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    block_tables: torch.Tensor, query_start: torch.Tensor, seq_lens: torch.Tensor, block_size: int,
+    layout: str, max_query_len: int, max_seq_len: int, scale: float | None = None,
+    causal: bool = True, window: int = 0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return attend_block_scaled(
+        q, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size, layout,
+        max_query_len=max_query_len, max_seq_len=max_seq_len, scale=scale, causal=causal,
+        window=window, return_lse=True)
+
+
+@_attend_block_scaled_op.register_fake
+def _(q, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size, layout,
+      max_query_len, max_seq_len, scale=None, causal=True, window=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
