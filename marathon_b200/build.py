@@ -26,6 +26,7 @@ SOURCES = [
     PKG / "csrc" / "rotary_axes.cu",
     PKG / "csrc" / "append_block_scaled.cu",
     PKG / "csrc" / "attend_block_scaled.cu",
+    PKG / "csrc" / "attend_rows.cu",
 ]
 HEADERS = [
     ROOT / "include" / "marathon_shift.h",

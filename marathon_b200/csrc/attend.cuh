@@ -51,12 +51,17 @@ struct AttendArgs {
   void* out;
   int64_t o_tok, o_head;
   float* lse;  // [rows, hq] or null
-  // keys are cut into splits of `chunk`; more than one: partial results
-  // part_o[row][head][split][D] and part_ml[row][head][split], joined afterwards
+  // Requests of at most few_rows (token, group) rows go to the few-rows kernel, the others to
+  // the many-rows one; each cuts the keys into splits of its own.  More than one: partial
+  // results acc [split][D] and (M, l) [split] for each (row, head), joined afterwards.
+  int few_rows;
   int chunk, nsplit;
+  int64_t cap;  // rows a (request, head) has in part_o, or 0: part_o goes by (row of q, head)
   float* part_o;
   float2* part_ml;
-  int few_rows;  // requests of at most this many (token, group) rows go to the few-rows kernel
+  int rchunk, rsplit;
+  float* rpart_o;  // by (row of q, head)
+  float2* rpart_ml;
   int zero_tail;
   int max_q;     // the caller's bound on a request's tokens
   uint32_t* err;

@@ -22,6 +22,9 @@
 namespace mshift {
 namespace serve {
 
+template <int D, typename T>
+cudaError_t launch_attend_rows(const AttendArgs& a, cudaStream_t stream);
+
 namespace {
 
 constexpr int kWarps = 4;
@@ -360,7 +363,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
     const int64_t row = rq.q0 + (m0 + m) / a.group;
     const int hq = h * a.group + (m0 + m) % a.group;
     if (a.nsplit > 1) {
-      const int64_t part = (row * a.hq + hq) * a.nsplit + split;
+      const int64_t part =
+          (a.cap ? (((int64_t)r * a.hk + h) * a.cap + m0 + m) : row * a.hq + hq) * a.nsplit + split;
       *reinterpret_cast<float4*>(a.part_o + part * D + d) = make_float4(x[0], x[1], x[2], x[3]);
       if (d == 0) a.part_ml[part] = make_float2(top, sum);
     } else {
@@ -376,31 +380,49 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
 }
 
 // o = sum_s 2^(M_s - M) acc_s / sum_s 2^(M_s - M) l_s over the splits of one (row, head);
-// a CTA for each, a thread for each dim.
-template <int D, typename T>
+// a CTA for each, a thread for each dim.  ROWS: of the many-rows kernel.
+template <int D, typename T, bool ROWS>
 __global__ void __launch_bounds__(D) attend_join_kernel(const AttendArgs a) {
   extern __shared__ float s_by[];
   __shared__ float s_red[2][D / 32];
-  const int64_t row = blockIdx.x / a.hq;
-  const int hq = blockIdx.x % a.hq, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int chunk = ROWS ? a.rchunk : a.chunk, nsplit = ROWS ? a.rsplit : a.nsplit;
+  const float* part_o = ROWS ? a.rpart_o : a.part_o;
+  const float2* part_ml = ROWS ? a.rpart_ml : a.part_ml;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= row_start(a.qs, a.reqs, a.rows)) return;
-  const int r = find_request(a.reqs, row, [&](int i) { return (long long)row_start(a.qs, i, a.rows); });
-  const Request rq = request_of(a, r, false);
-  if (row < rq.q0 || row >= rq.q0 + rq.n) return;
+  int64_t row;
+  int hq;
+  Request rq;
+  if (!ROWS && a.cap) {
+    const int64_t m = blockIdx.x % a.cap, rh = blockIdx.x / a.cap;
+    const int r = (int)(rh / a.hk);
+    rq = request_of(a, r, false);
+    if (m >= (int64_t)rq.n * a.group) return;
+    row = rq.q0 + m / a.group;
+    hq = (int)(rh % a.hk) * a.group + (int)(m % a.group);
+  } else {
+    row = blockIdx.x / a.hq;
+    hq = blockIdx.x % a.hq;
+    if (row >= row_start(a.qs, a.reqs, a.rows)) return;
+    const int r =
+        find_request(a.reqs, row, [&](int i) { return (long long)row_start(a.qs, i, a.rows); });
+    rq = request_of(a, r, false);
+    if (row < rq.q0 || row >= rq.q0 + rq.n) return;
+  }
+  if (((int64_t)rq.n * a.group > a.few_rows) != ROWS) return;
   const int2 see = seen(a, rq, rq.start + (row - rq.q0));
   // splits that hold a key of this row; at least one, for a row without keys
-  const int s0 = see.x / a.chunk, s1 = max((see.y + a.chunk - 1) / a.chunk, s0 + 1);
-  const int64_t part = blockIdx.x * (int64_t)a.nsplit;
+  const int s0 = see.x / chunk, s1 = max((see.y + chunk - 1) / chunk, s0 + 1);
+  const int64_t part = blockIdx.x * (int64_t)nsplit;
   float top = kNoKey;
-  for (int s = s0 + tid; s < s1; s += D) top = fmaxf(top, a.part_ml[part + s].x);
+  for (int s = s0 + tid; s < s1; s += D) top = fmaxf(top, part_ml[part + s].x);
   for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (lane == 0) s_red[0][warp] = top;
   __syncthreads();
   for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[0][w]);
   float sum = 0.0f;
   for (int s = s0 + tid; s < s1; s += D) {
-    const float2 ml = a.part_ml[part + s];
+    const float2 ml = part_ml[part + s];
     const float by = ex2(ml.x - top);
     s_by[s - s0] = by;
     sum = fmaf(ml.y, by, sum);
@@ -411,7 +433,7 @@ __global__ void __launch_bounds__(D) attend_join_kernel(const AttendArgs a) {
   sum = 0.0f;
   for (int w = 0; w < D / 32; ++w) sum += s_red[1][w];
   float x = 0.0f;
-  const float* src = a.part_o + (part + s0) * D + tid;
+  const float* src = part_o + (part + s0) * D + tid;
 #pragma unroll 8
   for (int s = 0; s < s1 - s0; ++s) x = fmaf(src[(int64_t)s * D], s_by[s], x);
   const bool any = top > kNoKey;
@@ -434,69 +456,95 @@ cudaError_t launch_few(const AttendArgs& a, int64_t most_rows, cudaStream_t stre
   return cudaGetLastError();
 }
 
-template <int D, typename T>
+template <int D, typename T, bool ROWS>
 cudaError_t launch_join(const AttendArgs& a, cudaStream_t stream) {
+  const int64_t grid = !ROWS && a.cap ? (int64_t)a.reqs * a.hk * a.cap : (int64_t)a.rows * a.hq;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.rows * a.hq));
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(D);
-  cfg.dynamicSmemBytes = sizeof(float) * a.nsplit;
+  cfg.dynamicSmemBytes = sizeof(float) * (ROWS ? a.rsplit : a.nsplit);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T>, a);
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T, ROWS>, a);
 }
 
 template <int D, typename T>
-cudaError_t launch_all(const AttendArgs& a, int64_t most_rows, cudaStream_t stream) {
+cudaError_t launch_all(const AttendArgs& a, cudaStream_t stream) {
+  const int64_t all = (int64_t)min(a.max_q, a.rows) * a.group;
+  const int64_t few = min(all, (int64_t)a.few_rows);
   // 8 rows a tile, or 16 where a request has more: twice the rows for the same codes
   cudaError_t e;
-  if constexpr (D == 256) {
-    e = launch_few<D, 1, T>(a, most_rows, stream);
-  } else {
-    e = most_rows <= 8 ? launch_few<D, 1, T>(a, most_rows, stream)
-                       : launch_few<D, 2, T>(a, most_rows, stream);
+  if constexpr (D == 256)
+    e = launch_few<D, 1, T>(a, few, stream);
+  else
+    e = few <= 8 ? launch_few<D, 1, T>(a, few, stream) : launch_few<D, 2, T>(a, few, stream);
+  if (e == cudaSuccess && a.nsplit > 1) e = launch_join<D, T, false>(a, stream);
+  if constexpr (D <= 128) {
+    if (e == cudaSuccess && all > a.few_rows) {
+      e = launch_attend_rows<D, T>(a, stream);
+      if (e == cudaSuccess && a.rsplit > 1) e = launch_join<D, T, true>(a, stream);
+    }
   }
-  if (e == cudaSuccess && a.nsplit > 1) e = launch_join<D, T>(a, stream);
   return e;
 }
 
 template <typename T>
 int attend_dispatch(const AttendArgs& a, int head_size, cudaStream_t stream) {
-  const int64_t most_rows = min((int64_t)min(a.max_q, a.rows) * a.group, (int64_t)a.few_rows);
   cudaError_t e;
   switch (head_size) {
-    case 64: e = launch_all<64, T>(a, most_rows, stream); break;
-    case 128: e = launch_all<128, T>(a, most_rows, stream); break;
-    case 256: e = launch_all<256, T>(a, most_rows, stream); break;
+    case 64: e = launch_all<64, T>(a, stream); break;
+    case 128: e = launch_all<128, T>(a, stream); break;
+    case 256: e = launch_all<256, T>(a, stream); break;
     default: return MSHIFT_EUNSUPPORTED;
   }
   return e == cudaSuccess ? MSHIFT_OK : cuda_fail(e);
 }
 
 constexpr int kMaxSplits = 1024;
+constexpr int kFewRows = 32;  // rows of a request up to which the few-rows kernel is the faster
 
-// Tokens of a split.  Enough splits that the CTAs of all requests, heads and tiles fill
-// the GPU's 148 SMs a few times over, but no split so short that its start-up shows.
-int chunk_for(int64_t units, int max_len) {
-  const int64_t want = 148 * 8;
-  int64_t splits = (want + units - 1) / units;
-  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
-  int64_t chunk = ((int64_t)max_len + splits - 1) / splits;
-  chunk = chunk < 256 ? 256 : chunk > 2048 ? 2048 : chunk;
-  const int64_t least = ((int64_t)max_len + kMaxSplits - 1) / kMaxSplits;
-  if (chunk < least) chunk = least;
-  return (int)((chunk + 63) / 64 * 64);
+// Tokens of a split, a multiple of 128, between least and most.  Enough splits that the CTAs of
+// all units fill `want` places, but none so short that its start-up shows.
+int chunk_for(int64_t units, int64_t want, int max_len, int64_t least, int64_t most) {
+  const int64_t splits = units > 0 ? (want + units - 1) / units : 1;
+  int64_t chunk = splits <= 1 ? most : ((int64_t)max_len + splits - 1) / splits;
+  chunk = chunk < least ? least : chunk > most ? most : chunk;
+  const int64_t floor = ((int64_t)max_len + kMaxSplits - 1) / kMaxSplits;
+  if (chunk < floor) chunk = floor;
+  return (int)((chunk + 127) / 128 * 128);
 }
 
-void plan(int32_t rows, int32_t hq, int32_t hk, int32_t reqs, int32_t max_q, int32_t max_len,
-          int* chunk, int* nsplit) {
-  const int64_t most = (int64_t)(max_q < rows ? max_q : rows) * (hq / hk);
-  const int64_t tiles = most <= 8 ? 1 : (most + 15) / 16;
-  *chunk = chunk_for((int64_t)reqs * hk * tiles, max_len);
-  *nsplit = max_len > 0 ? (max_len + *chunk - 1) / *chunk : 1;
+struct Plan {
+  int few_rows, chunk, nsplit, rchunk, rsplit;
+  int64_t cap;
+  int64_t parts, rparts;  // partial results of each kernel
+};
+
+Plan plan(int32_t rows, int32_t hq, int32_t hk, int32_t head_size, int32_t reqs, int32_t max_q,
+          int32_t max_len) {
+  Plan p{};
+  const int64_t group = hq / hk, all = (int64_t)(max_q < rows ? max_q : rows) * group;
+  p.few_rows = head_size > 128 ? INT32_MAX : kFewRows;
+  const int64_t few = all < p.few_rows ? all : p.few_rows;
+  const int64_t tiles = few <= 8 ? 1 : (few + 15) / 16;
+  p.chunk = chunk_for((int64_t)reqs * hk * tiles, 148 * 8, max_len, 256, 2048);
+  p.nsplit = max_len > 0 ? (int)(((int64_t)max_len + p.chunk - 1) / p.chunk) : 1;
+  p.cap = (int64_t)reqs * hk * few <= (int64_t)rows * hq ? few : 0;
+  if (p.nsplit > 1) p.parts = (p.cap ? (int64_t)reqs * hk * p.cap : (int64_t)rows * hq) * p.nsplit;
+  p.rchunk = 1 << 30;
+  p.rsplit = 1;
+  if (all > p.few_rows) {
+    const int64_t items = (int64_t)rows * group / 256 + reqs;
+    p.rchunk = chunk_for(items * hk, 148 * 4, max_len, 1024, 1 << 30);
+    p.rsplit = max_len > 0 ? (int)(((int64_t)max_len + p.rchunk - 1) / p.rchunk) : 1;
+    if (p.rsplit > 1) p.rparts = (int64_t)rows * hq * p.rsplit;
+  }
+  return p;
 }
 
 }  // namespace
@@ -511,9 +559,8 @@ int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk, int32_t he
       max_query_len < 0 || max_seq_len < 0)
     return -1;
   if (rows == 0 || reqs == 0) return 0;
-  int chunk, nsplit;
-  mshift::serve::plan(rows, hq, hk, reqs, max_query_len, max_seq_len, &chunk, &nsplit);
-  return nsplit > 1 ? (int64_t)rows * hq * nsplit * (head_size + 2) * 4 : 0;
+  const auto p = mshift::serve::plan(rows, hq, hk, head_size, reqs, max_query_len, max_seq_len);
+  return (p.parts + p.rparts) * (head_size + 2) * 4;
 }
 
 int mshift_attend_block_scaled(
@@ -543,11 +590,11 @@ int mshift_attend_block_scaled(
   if (odd(q) || odd(k_base) || odd(v_base) || q_tok % 8 || q_head % 8 || paged->blk_stride % 16 ||
       paged->off_stride % 16 || paged->head_stride % 16)
     return MSHIFT_EINVAL;
-  int chunk, nsplit;
-  plan(rows, hq, paged->heads, reqs, max_query_len, max_seq_len, &chunk, &nsplit);
-  const int64_t parts = (int64_t)rows * hq * nsplit;
-  if (nsplit > 1 && (workspace == nullptr || odd(workspace) ||
-                     workspace_bytes < parts * (paged->head_size + 2) * 4))
+  const Plan p = plan(rows, hq, paged->heads, paged->head_size, reqs, max_query_len, max_seq_len);
+  const int64_t d = paged->head_size;
+  if (p.parts + p.rparts > 0 &&
+      (workspace == nullptr || odd(workspace) ||
+       workspace_bytes < (p.parts + p.rparts) * (d + 2) * 4))
     return MSHIFT_EINVAL;
   AttendArgs a{};
   a.q = q;
@@ -584,11 +631,16 @@ int mshift_attend_block_scaled(
   a.o_tok = o_tok;
   a.o_head = o_head;
   a.lse = lse;
-  a.chunk = chunk;
-  a.nsplit = nsplit;
+  a.few_rows = p.few_rows;
+  a.chunk = p.chunk;
+  a.nsplit = p.nsplit;
+  a.cap = p.cap;
+  a.rchunk = p.rchunk;
+  a.rsplit = p.rsplit;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + parts * paged->head_size);
-  a.few_rows = INT32_MAX;
+  a.rpart_o = a.part_o + p.parts * d;
+  a.part_ml = reinterpret_cast<float2*>(a.rpart_o + p.rparts * d);
+  a.rpart_ml = a.part_ml + p.parts;
   a.zero_tail = zero_tail;
   a.max_q = max_query_len;
   a.err = err;

@@ -1,0 +1,652 @@
+// attend_rows.cu — attention over a block-scaled e4m3 paged cache: the kernel for
+// many query rows (chunks and prefills), on the fifth-generation tensor cores.
+//
+// A CTA has 256 (token, head of the group) rows of one request and KV head, as two tiles of
+// 128, and walks the keys they see in tiles of 128 (attend.cuh has the mathematics):
+//     S_t = Q_t K^T        tcgen05.mma 128 x 128 x D, Q and K f16 in shared memory, S in TMEM
+//     P_t = 2^(t - M)      a thread a row: TMEM -> registers -> f16 -> TMEM, in place of S
+//     O_t += P_t V         tcgen05.mma 128 x D x 128, P from TMEM, V f16 in shared memory
+// Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in,
+// warp 12 issues the matrix products.  While one tile's softmax runs, the other tile's products
+// do, so neither waits for the other in the steady state.
+//
+// e4m3 has no matrix product with f16, so the loaders convert: 16 codes a 16-byte load,
+// exactly, into the 128-byte-swizzled tiles that the descriptors name.  K and V have the
+// same layout in shared memory (rows of tokens, 64 dims a swizzle atom); K is read with its dims as the
+// contraction (K-major), V with its tokens (MN-major), so no tile is transposed.
+// A code is converted once for 256 rows.
+//
+// TMEM columns: S (then P) of tile 0 at 0, of tile 1 at 128, O of tile 0 at 256, of tile 1 at 256 + D.
+// O is rescaled in place when a row's maximum passes its reference by 2^8, which is rare after
+// the first tiles; S_t of a key tile is complete only after the product P_t V of
+// the one before (one thread issues them in that order and the commit covers both),
+// so the rescaling thread needs no further barrier.
+//
+// Registers: 512 threads are launched with 128 each; the softmax warps take 184
+// (a row's 128 scores at once), the loaders 96 (two tiles' codes in flight) and the rest 48,
+// which is the launch's sum.
+//
+// Every wait is bounded: one that runs out sets MSHIFT_EBIT_TIMEOUT, every role leaves
+// its loop, issued products are waited for, TMEM is freed and the CTA returns.
+#include "attend.cuh"
+
+namespace mshift {
+namespace serve {
+namespace {
+
+constexpr int kTile = 128;  // keys of a tile, rows of a row tile
+constexpr int kCta = 512;
+constexpr int kScaleRing = 4;
+constexpr uint32_t kRounds = 1u << 18;  // try_wait rounds of a wait
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
+// False once the wait, or another role's, has run out.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* gone,
+                                         uint32_t* err) {
+  if (bar_try(b, parity)) return true;
+  for (uint32_t i = 0; i < kRounds; ++i) {
+    if (bar_try(b, parity)) return true;
+    if (*gone) return false;
+  }
+  *gone = 1;
+  flag(err, MSHIFT_EBIT_TIMEOUT);
+  return false;
+}
+
+__device__ __forceinline__ void commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(b))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_smem() {  // generic stores, then the tensor core's reads
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Shared-memory descriptor of a 128-byte-swizzled tile: groups of 8 rows are 1,024 bytes
+// apart; `lead` is the distance between 64-element columns where they are the rows of
+// the operand (MN-major), unused otherwise.
+__device__ __forceinline__ uint64_t descriptor(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(lead >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f16 x f16 -> f32, M = 128; bit 16: B is MN-major.
+__device__ constexpr uint32_t instruction(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                         bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+
+// 32 columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_loaded() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// What was loaded may be used from here on: keeps the compiler from moving arithmetic on the
+// registers to before the wait.
+template <int N>
+__device__ __forceinline__ void tmem_use(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_stored() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <int D>
+struct alignas(1024) Smem {
+  static constexpr int kBytes = kTile * D * 2;  // an f16 tile
+  uint8_t q[2][kBytes];
+  uint8_t k[2][kBytes];
+  uint8_t v[2][kBytes];
+  float4 scale[kScaleRing][kTile];  // of each key: ks, log2 vs, 1 / vs
+  long long at[2][kTile];           // byte offset of each key in the cache, -1: not read
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[kScaleRing], s_full[2],
+      p_full[2], done;
+  uint32_t tmem;
+  int gone;
+};
+
+// Byte offset of 16-byte chunk `c` (8 dims) of row `row` in a swizzled tile.
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int row, int c) {
+  return (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+
+// Keys [lo, hi) of this CTA, from tile-aligned `first`, in `tiles` tiles.
+struct Span {
+  int lo, hi, first, tiles;
+};
+
+template <int D>
+__device__ __forceinline__ void load_codes(const uint8_t* base, const long long* at, int part,
+                                           int row0, uint4* w) {
+  constexpr int kPer = D / 16, kStep = 128 / kPer;
+#pragma unroll
+  for (int i = 0; i < kTile / kStep; ++i) {
+    const long long off = at[row0 + i * kStep];
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (off >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(base + off + part * 16));
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_f16(uint8_t* tile, int part, int row0, const uint4* w) {
+  constexpr int kPer = D / 16, kStep = 128 / kPer;
+#pragma unroll
+  for (int i = 0; i < kTile / kStep; ++i) {
+    const int row = row0 + i * kStep;
+    uint32_t f[8];
+    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = e4m3x2_to_f16x2((uint16_t)x[e]);
+      f[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(x[e] >> 16));
+    }
+    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part)) = make_uint4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + 1)) =
+        make_uint4(f[4], f[5], f[6], f[7]);
+  }
+}
+
+template <int D, bool PAGE16>
+__device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int r, int h, const Span sp) {
+  const int tid = threadIdx.x - 256;
+  constexpr int kPer = D / 16;
+  const int part = tid % kPer, row0 = tid / kPer;
+  const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
+  const uint8_t* kh = a.k + h * a.head;
+  const uint8_t* vh = a.v + h * a.head;
+  constexpr int kLoads = kTile / (128 / kPer);
+  uint4 kw[kLoads], vw[kLoads];
+
+  // thread t finds key t of a tile: its place and its block's scales
+  auto place = [&](int it, long long& off, float4& sc) {
+    const int key = sp.first + it * kTile + tid;
+    off = -1;
+    sc = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    if (it >= sp.tiles) return;
+    // PAGE16 reads the scales of 16 keys at the first of them, which may itself be outside
+    if (PAGE16 ? (key | 15) < sp.lo || (key & ~15) >= sp.hi : key < sp.lo || key >= sp.hi) return;
+    const int col = key / a.bs;
+    const int b = table[col];
+    if (b < 0 || b >= a.num_blocks) {
+      flag(a.err, MSHIFT_EBIT_SLOT);
+      return;
+    }
+    if (key >= sp.lo && key < sp.hi) off = b * a.blk + (key - col * a.bs) * a.off;
+    const float vs = fmaxf(a.vs[b * a.vs_blk + h * a.vs_head], kScaleFloor);
+    sc = make_float4(a.ks[b * a.ks_blk + h * a.ks_head], __log2f(vs), __frcp_rn(vs), 0.0f);
+  };
+  auto publish = [&](int it, long long off, const float4& sc) {
+    s.at[it & 1][tid] = off;
+    s.scale[it % kScaleRing][tid] = sc;
+    bar_arrive(&s.scale_full[it % kScaleRing]);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  };
+
+  long long off;
+  float4 sc;
+  place(0, off, sc);
+  publish(0, off, sc);
+  load_codes<D>(kh, s.at[0], part, row0, kw);
+  for (int it = 0; it < sp.tiles; ++it) {
+    const int st = it & 1;
+    const uint32_t free = ((it >> 1) & 1) ^ 1;
+    load_codes<D>(vh, s.at[it & 1], part, row0, vw);
+    place(it + 1, off, sc);
+    bool ok = bar_wait(&s.k_empty[st], free, &s.gone, a.err);
+    if (ok) {
+      store_f16<D>(s.k[st], part, row0, kw);
+      fence_smem();
+      bar_arrive(&s.k_full[st]);
+    }
+    // every loader meets here even after a wait ran out, or the others would hang
+    if (it + 1 < sp.tiles) {
+      publish(it + 1, off, sc);
+      load_codes<D>(kh, s.at[(it + 1) & 1], part, row0, kw);
+    }
+    ok = ok && bar_wait(&s.v_empty[st], free, &s.gone, a.err);
+    if (ok) {
+      store_f16<D>(s.v[st], part, row0, vw);
+      fence_smem();
+      bar_arrive(&s.v_full[st]);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void issuer(const AttendArgs& a, Smem<D>& s, int tiles, bool two) {
+  constexpr uint32_t kScore = instruction(kTile, false), kValue = instruction(D, true);
+  const uint32_t tmem = s.tmem;
+  const uint32_t q0 = smem_u32(s.q[0]), k0 = smem_u32(s.k[0]), v0 = smem_u32(s.v[0]);
+  auto scores = [&](int t, int st) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {  // 16 dims: 32 bytes of a 128-byte row
+      const uint32_t in = (d >> 2) * (kTile * 128) + (d & 3) * 32;
+      mma_smem(tmem + t * kTile, descriptor(q0 + t * Smem<D>::kBytes + in, 16),
+               descriptor(k0 + st * Smem<D>::kBytes + in, 16), kScore, d > 0);
+    }
+    commit(&s.s_full[t]);
+  };
+  bool ok = bar_wait(&s.q_full, 0, &s.gone, a.err) && bar_wait(&s.k_full[0], 0, &s.gone, a.err);
+  fence_after();
+  if (ok) {
+    scores(0, 0);
+    if (two) scores(1, 0);
+    commit(&s.k_empty[0]);
+  }
+  for (int it = 0; ok && it < tiles; ++it) {
+    const int st = it & 1, nx = (it + 1) & 1;
+    ok = bar_wait(&s.v_full[st], (it >> 1) & 1, &s.gone, a.err);
+    for (int t = 0; ok && t < (two ? 2 : 1); ++t) {
+      ok = bar_wait(&s.p_full[t], it & 1, &s.gone, a.err);
+      if (!ok) break;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)  // 16 keys: two groups of 8 rows
+        mma_tmem(tmem + 256 + t * D, tmem + t * kTile + k * 8,
+                 descriptor(v0 + st * Smem<D>::kBytes + k * 2048, kTile * 128), kValue,
+                 it > 0 || k > 0);
+      if (it + 1 < tiles) {
+        if (t == 0) ok = bar_wait(&s.k_full[nx], ((it + 1) >> 1) & 1, &s.gone, a.err);
+        if (!ok) break;
+        fence_after();
+        scores(t, nx);
+      }
+    }
+    if (!ok) break;
+    commit(&s.v_empty[st]);
+    if (it + 1 < tiles) commit(&s.k_empty[nx]);
+  }
+  // also after a wait ran out: what was issued completes before TMEM is freed
+  commit(&s.done);
+}
+
+// Rows 32 * (warp % 4) + lane of tile t.
+template <int D, bool PAGE16, typename T>
+__device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const Request& rq, int h,
+                                        int m0, int split, const Span sp, int all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+  const int m = m0 + t * kTile + row;
+  const bool live = m < all;
+  const int64_t tok = rq.q0 + (live ? m / a.group : 0);
+  const int hq = h * a.group + (live ? m % a.group : 0);
+  int2 see = live ? seen(a, rq, rq.start + m / a.group) : make_int2(0, 0);
+  see.x = max(see.x, sp.lo);
+  see.y = min(see.y, sp.hi);
+
+  // the query row: f16 after a power of two
+  float rf = a.scale_log2;
+  {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.q_tok +
+                                                      hq * a.q_head);
+    float top = 0.0f;
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+      float f[8];
+      Elem<T>::unpack(w.x, f);
+      Elem<T>::unpack(w.y, f + 2);
+      Elem<T>::unpack(w.z, f + 4);
+      Elem<T>::unpack(w.w, f + 6);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+    }
+    int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+    if (e2 < -126 || e2 > 126) e2 = 0;
+    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+    rf *= __uint_as_float((uint32_t)(127 + e2) << 23);
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+      float f[8];
+      Elem<T>::unpack(w.x, f);
+      Elem<T>::unpack(w.y, f + 2);
+      Elem<T>::unpack(w.z, f + 4);
+      Elem<T>::unpack(w.w, f + 6);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= down;
+      *reinterpret_cast<uint4*>(s.q[t] + tile_at<D>(row, c)) =
+          make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]),
+                     pack_f16x2(f[6], f[7]));
+    }
+    fence_smem();
+    bar_arrive(&s.q_full);
+  }
+  if (m0 + t * kTile >= all) return;  // a tile without rows
+
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const uint32_t s_at = s.tmem + lanes + t * kTile, o_at = s.tmem + lanes + 256 + t * D;
+  float M = kNoKey, l = 0.0f;
+  bool ok = true;
+  for (int it = 0; it < sp.tiles; ++it) {
+    const int key0 = sp.first + it * kTile;
+    ok = bar_wait(&s.scale_full[it % kScaleRing], (it / kScaleRing) & 1, &s.gone, a.err);
+    ok = ok && bar_wait(&s.s_full[t], it & 1, &s.gone, a.err);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    fence_after();
+    uint32_t x[kTile];
+#pragma unroll
+    for (int c = 0; c < kTile; c += 32) tmem_load32(s_at + c, x + c);
+    tmem_loaded();
+    tmem_use<kTile>(x);
+
+    const float4* sc = s.scale[it % kScaleRing];
+    float top = M;
+    if constexpr (PAGE16) {  // one scale for 16 keys
+#pragma unroll
+      for (int b = 0; b < kTile / 16; ++b) {
+        const float4 y = sc[b * 16];
+        const float by = rf * y.x;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          x[b * 16 + e] = __float_as_uint(fmaf(__uint_as_float(x[b * 16 + e]), by, y.y));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kTile; ++e) {
+        const float4 y = sc[e];
+        x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), rf * y.x, y.y));
+      }
+    }
+    const bool whole = see.x <= key0 && see.y >= key0 + kTile;
+    if (!__all_sync(0xffffffffu, whole)) {
+      const int lo = see.x - key0, hi = see.y - key0;
+#pragma unroll
+      for (int e = 0; e < kTile; ++e)
+        if (e < lo || e >= hi) x[e] = __float_as_uint(-INFINITY);
+    }
+#pragma unroll
+    for (int e = 0; e < kTile; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+    const bool passed = top > M + kLazy;
+    if (__any_sync(0xffffffffu, passed)) {
+      const float by = passed ? ex2(M - top) : 1.0f;
+      if (passed) M = top;
+      l *= by;
+      if (it > 0) {
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o_at + c, o);
+          tmem_loaded();
+          tmem_use<32>(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+          tmem_store32(o_at + c, o);
+        }
+      }
+    }
+    uint32_t p[kTile / 2];
+    if constexpr (PAGE16) {
+#pragma unroll
+      for (int b = 0; b < kTile / 16; ++b) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = ex2(__uint_as_float(x[b * 16 + e]) - M);
+          const float p1 = ex2(__uint_as_float(x[b * 16 + e + 1]) - M);
+          sum += p0 + p1;
+          p[b * 8 + e / 2] = pack_f16x2(p0, p1);
+        }
+        l = fmaf(sum, sc[b * 16].z, l);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kTile; e += 2) {
+        const float p0 = ex2(__uint_as_float(x[e]) - M);
+        const float p1 = ex2(__uint_as_float(x[e + 1]) - M);
+        l = fmaf(p0, sc[e].z, l);
+        l = fmaf(p1, sc[e + 1].z, l);
+        p[e / 2] = pack_f16x2(p0, p1);
+      }
+    }
+    tmem_store32(s_at, p);
+    tmem_store32(s_at + 32, p + 32);
+    tmem_stored();
+    fence_before();
+    bar_arrive(&s.p_full[t]);
+  }
+
+  if (ok) ok = __all_sync(0xffffffffu, bar_wait(&s.done, 0, &s.gone, a.err));
+  if (!ok || s.gone) return;
+  fence_after();
+  const bool any = M > kNoKey;
+  const float by = any ? 1.0f / l : 0.0f;
+  const int64_t part = (tok * a.hq + hq) * a.rsplit + split;
+#pragma unroll
+  for (int c = 0; c < D; c += 32) {
+    uint32_t o[32];
+    tmem_load32(o_at + c, o);
+    tmem_loaded();
+    tmem_use<32>(o);
+    if (!live) continue;
+    if (a.rsplit > 1) {
+      float4* dst = reinterpret_cast<float4*>(a.rpart_o + part * D + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                             __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+    } else {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_tok + hq * a.o_head + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = any ? __uint_as_float(o[8 * e + i]) * by : 0.0f;
+        dst[e] = make_uint4(Elem<T>::pack(f), Elem<T>::pack(f + 2), Elem<T>::pack(f + 4),
+                            Elem<T>::pack(f + 6));
+      }
+    }
+  }
+  if (!live) return;
+  if (a.rsplit > 1)
+    a.rpart_ml[part] = make_float2(M, l);
+  else if (a.lse != nullptr)
+    a.lse[tok * a.hq + hq] = any ? (M + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// Rows without a key in this CTA's span: an empty part, or zeros.
+template <int D, typename T>
+__device__ __forceinline__ void nothing(const AttendArgs& a, const Request& rq, int h, int m0,
+                                        int split, int all) {
+  for (int i = threadIdx.x; i < min(2 * kTile, all - m0); i += kCta) {
+    const int m = m0 + i;
+    const int64_t tok = rq.q0 + m / a.group;
+    const int hq = h * a.group + m % a.group;
+    if (a.rsplit > 1) {
+      a.rpart_ml[(tok * a.hq + hq) * a.rsplit + split] = make_float2(kNoKey, 0.0f);
+      continue;
+    }
+    T* dst = static_cast<T*>(a.out) + tok * a.o_tok + hq * a.o_head;
+    for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+    if (a.lse != nullptr) a.lse[tok * a.hq + hq] = -INFINITY;
+  }
+}
+
+template <int D, bool PAGE16, typename T>
+__global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a, int items) {
+  extern __shared__ uint8_t raw[];
+  Smem<D>& s = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5;
+  int64_t id = blockIdx.x;
+  const int h = (int)(id % a.hk);
+  id /= a.hk;
+  const int split = (int)(id % a.rsplit);
+  id /= a.rsplit;
+  // a request's later rows see more keys: the longest tiles first
+  const long long item = items - 1 - id;
+  // a request of n rows has at most ceil(n / 256) tiles, and floor(q_r / 256) + r numbers
+  // them without a scan over the requests
+  const int r = find_request(a.reqs, item, [&](int i) {
+    return (long long)row_start(a.qs, i, a.rows) * a.group / (2 * kTile) + i;
+  });
+  const Request rq = request_of(a, r, threadIdx.x == 0 && h == 0 && split == 0);
+  const long long base = (long long)rq.q0 * a.group / (2 * kTile) + r;
+  const long long rows = (long long)rq.n * a.group;
+  if (item < base || rows <= a.few_rows || (item - base) * 2 * kTile >= rows) return;
+  const int m0 = (int)(item - base) * 2 * kTile, all = (int)rows;
+  const int last_m = min(m0 + 2 * kTile, all) - 1;
+  Span sp;
+  {
+    const int2 head = seen(a, rq, max(rq.start + m0 / a.group, 0ll));
+    const int2 last = seen(a, rq, rq.start + last_m / a.group);
+    sp.lo = max(head.x, split * a.rchunk);
+    sp.hi = (int)min((long long)last.y, (long long)split * a.rchunk + a.rchunk);
+    sp.first = sp.lo / kTile * kTile;
+    sp.tiles = sp.hi > sp.lo ? (sp.hi - sp.first + kTile - 1) / kTile : 0;
+  }
+  if (sp.tiles == 0) {
+    nothing<D, T>(a, rq, h, m0, split, all);
+    return;
+  }
+  const bool two = m0 + kTile < all;
+
+  if (threadIdx.x == 0) {
+    bar_init(&s.q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.k_full[i], 128);
+      bar_init(&s.k_empty[i], 1);
+      bar_init(&s.v_full[i], 128);
+      bar_init(&s.v_empty[i], 1);
+      bar_init(&s.s_full[i], 1);
+      bar_init(&s.p_full[i], 128);
+    }
+    for (int i = 0; i < kScaleRing; ++i) bar_init(&s.scale_full[i], 128);
+    bar_init(&s.done, 1);
+    s.gone = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(&s.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+
+  // 256 * 184 + 128 * 96 + 128 * 48 = 512 * 128 registers
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    softmax<D, PAGE16, T>(a, s, rq, h, m0, split, sp, all);
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    loader<D, PAGE16>(a, s, r, h, sp);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 12) {
+      if ((threadIdx.x & 31) == 0) {
+        issuer<D>(a, s, sp.tiles, two);
+        // after a wait that ran out nobody else waits for the products
+        for (uint32_t i = 0; i < kRounds && !bar_try(&s.done, 0); ++i) {
+        }
+      }
+      __syncwarp();
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s.tmem));
+}
+
+template <int D, bool PAGE16, typename T>
+cudaError_t launch(const AttendArgs& a, int items, cudaStream_t stream) {
+  const int bytes = (int)sizeof(Smem<D>) + 1024;
+  const auto fn = attend_rows_kernel<D, PAGE16, T>;
+  // the roles' register shares add up to 512 * 128: a build that launched with fewer would
+  // wait for the difference for good
+  static const int regs = [fn] {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, fn) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs != 128) return cudaErrorLaunchOutOfResources;
+  // every call: the attribute belongs to the current device, and setting it is cheap
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  const int64_t grid = (int64_t)items * a.rsplit * a.hk;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  fn<<<(unsigned)grid, kCta, bytes, stream>>>(a, items);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+template <int D, typename T>
+cudaError_t launch_attend_rows(const AttendArgs& a, cudaStream_t stream) {
+  const int items = (int)((int64_t)a.rows * a.group / (2 * kTile)) + a.reqs;
+  return a.bs % 16 == 0 ? launch<D, true, T>(a, items, stream) : launch<D, false, T>(a, items, stream);
+}
+
+template cudaError_t launch_attend_rows<64, __nv_bfloat16>(const AttendArgs&, cudaStream_t);
+template cudaError_t launch_attend_rows<64, __half>(const AttendArgs&, cudaStream_t);
+template cudaError_t launch_attend_rows<128, __nv_bfloat16>(const AttendArgs&, cudaStream_t);
+template cudaError_t launch_attend_rows<128, __half>(const AttendArgs&, cudaStream_t);
+
+}  // namespace serve
+}  // namespace mshift
