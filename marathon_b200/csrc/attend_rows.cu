@@ -22,8 +22,8 @@
 // the one before (one thread issues them in that order and the commit covers both),
 // so the rescaling thread needs no further barrier.
 //
-// Registers: 512 threads are launched with 128 each; the softmax warps take 184
-// (a row's 128 scores at once), the loaders 96 (two tiles' codes in flight) and the rest 48,
+// Registers: 512 threads are launched with 128 each; the softmax warps take 176
+// (64 scores of a row at once), the loaders 112 (two tiles' codes in flight) and the rest 48,
 // which is the launch's sum.
 //
 // Every wait is bounded: one that runs out sets MSHIFT_EBIT_TIMEOUT, every role leaves
@@ -35,6 +35,7 @@ namespace serve {
 namespace {
 
 constexpr int kTile = 128;  // keys of a tile, rows of a row tile
+constexpr int kHalf = 64;   // keys whose scores a softmax thread holds at once
 constexpr int kCta = 512;
 constexpr int kScaleRing = 4;
 constexpr uint32_t kRounds = 1u << 18;  // try_wait rounds of a wait
@@ -48,14 +49,20 @@ __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
 __device__ __forceinline__ void bar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
+// One arrival for a warp whose lanes have all fenced what they wrote: a barrier takes them
+// one by one.
+__device__ __forceinline__ void warp_arrive(uint64_t* b) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
 __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_u32(b)), "r"(parity), "r"(20000u)
+      : "r"(smem_u32(b)), "r"(parity)
       : "memory");
   return ok != 0;
 }
@@ -129,6 +136,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
         "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -153,6 +168,33 @@ __device__ __forceinline__ void tmem_use(uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_stored() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 template <int D>
@@ -205,9 +247,12 @@ __device__ __forceinline__ void store_f16(uint8_t* tile, int part, int row0, con
       f[2 * e] = e4m3x2_to_f16x2((uint16_t)x[e]);
       f[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(x[e] >> 16));
     }
-    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part)) = make_uint4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + 1)) =
-        make_uint4(f[4], f[5], f[6], f[7]);
+    // eight neighbouring lanes store at once: the lanes of the second 64 dims, whose rows lie
+    // in the same banks, take their two chunks in the other order
+    const bool swap = part >= 4;
+    const uint4 x0 = make_uint4(f[0], f[1], f[2], f[3]), x1 = make_uint4(f[4], f[5], f[6], f[7]);
+    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + swap)) = swap ? x1 : x0;
+    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + !swap)) = swap ? x0 : x1;
   }
 }
 
@@ -222,58 +267,72 @@ __device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int r, i
   constexpr int kLoads = kTile / (128 / kPer);
   uint4 kw[kLoads], vw[kLoads];
 
-  // thread t finds key t of a tile: its place and its block's scales
-  auto place = [&](int it, long long& off, float4& sc) {
+  // Thread t finds key t of a tile, in three steps an iteration apart, so that none waits
+  // for the one before: its block, the block's scales, and their entry in shared memory.
+  auto block_of = [&](int it) -> int {
     const int key = sp.first + it * kTile + tid;
-    off = -1;
-    sc = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-    if (it >= sp.tiles) return;
     // PAGE16 reads the scales of 16 keys at the first of them, which may itself be outside
-    if (PAGE16 ? (key | 15) < sp.lo || (key & ~15) >= sp.hi : key < sp.lo || key >= sp.hi) return;
-    const int col = key / a.bs;
-    const int b = table[col];
-    if (b < 0 || b >= a.num_blocks) {
-      flag(a.err, MSHIFT_EBIT_SLOT);
-      return;
-    }
-    if (key >= sp.lo && key < sp.hi) off = b * a.blk + (key - col * a.bs) * a.off;
-    const float vs = fmaxf(a.vs[b * a.vs_blk + h * a.vs_head], kScaleFloor);
-    sc = make_float4(a.ks[b * a.ks_blk + h * a.ks_head], __log2f(vs), __frcp_rn(vs), 0.0f);
+    if (it >= sp.tiles ||
+        (PAGE16 ? (key | 15) < sp.lo || (key & ~15) >= sp.hi : key < sp.lo || key >= sp.hi))
+      return -1;
+    const int b = table[key / a.bs];
+    if (b >= 0 && b < a.num_blocks) return b;
+    flag(a.err, MSHIFT_EBIT_SLOT);
+    return -1;
   };
-  auto publish = [&](int it, long long off, const float4& sc) {
-    s.at[it & 1][tid] = off;
-    s.scale[it % kScaleRing][tid] = sc;
-    bar_arrive(&s.scale_full[it % kScaleRing]);
+  auto scales_of = [&](int b, float& ks, float& vs) {
+    if (b < 0) return;
+    ks = a.ks[b * a.ks_blk + h * a.ks_head];
+    vs = a.vs[b * a.vs_blk + h * a.vs_head];
+  };
+  auto publish = [&](int it, int b, float ks, float vs) {
+    const int key = sp.first + it * kTile + tid;
+    vs = fmaxf(vs, kScaleFloor);
+    s.at[it & 1][tid] =
+        b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + key % a.bs * a.off : -1ll;
+    s.scale[it % kScaleRing][tid] = b >= 0 ? make_float4(ks, __log2f(vs), __frcp_rn(vs), 0.0f)
+                                           : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    warp_arrive(&s.scale_full[it % kScaleRing]);
     asm volatile("bar.sync 1, 128;" ::: "memory");
   };
 
-  long long off;
-  float4 sc;
-  place(0, off, sc);
-  publish(0, off, sc);
+  float ks1 = 0.0f, vs1 = 0.0f;
+  int b1 = block_of(0), b2 = block_of(1);
+  scales_of(b1, ks1, vs1);
+  publish(0, b1, ks1, vs1);
   load_codes<D>(kh, s.at[0], part, row0, kw);
+  load_codes<D>(vh, s.at[0], part, row0, vw);
+  b1 = b2;
+  scales_of(b1, ks1, vs1);
+  b2 = block_of(2);
+  bool ok = true;
   for (int it = 0; it < sp.tiles; ++it) {
     const int st = it & 1;
     const uint32_t free = ((it >> 1) & 1) ^ 1;
-    load_codes<D>(vh, s.at[it & 1], part, row0, vw);
-    place(it + 1, off, sc);
-    bool ok = bar_wait(&s.k_empty[st], free, &s.gone, a.err);
+    const bool more = it + 1 < sp.tiles;
+    ok = ok && bar_wait(&s.k_empty[st], free, &s.gone, a.err);
+    ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       store_f16<D>(s.k[st], part, row0, kw);
       fence_smem();
-      bar_arrive(&s.k_full[st]);
+      warp_arrive(&s.k_full[st]);
     }
     // every loader meets here even after a wait ran out, or the others would hang
-    if (it + 1 < sp.tiles) {
-      publish(it + 1, off, sc);
+    if (more) {
+      publish(it + 1, b1, ks1, vs1);
       load_codes<D>(kh, s.at[(it + 1) & 1], part, row0, kw);
+      b1 = b2;
+      scales_of(b1, ks1, vs1);
+      b2 = block_of(it + 3);
     }
     ok = ok && bar_wait(&s.v_empty[st], free, &s.gone, a.err);
+    ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       store_f16<D>(s.v[st], part, row0, vw);
       fence_smem();
-      bar_arrive(&s.v_full[st]);
+      warp_arrive(&s.v_full[st]);
     }
+    if (more) load_codes<D>(vh, s.at[(it + 1) & 1], part, row0, vw);
   }
 }
 
@@ -373,7 +432,7 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
                      pack_f16x2(f[6], f[7]));
     }
     fence_smem();
-    bar_arrive(&s.q_full);
+    warp_arrive(&s.q_full);
   }
   if (m0 + t * kTile >= all) return;  // a tile without rows
 
@@ -388,86 +447,112 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     fence_after();
-    uint32_t x[kTile];
-#pragma unroll
-    for (int c = 0; c < kTile; c += 32) tmem_load32(s_at + c, x + c);
-    tmem_loaded();
-    tmem_use<kTile>(x);
-
     const float4* sc = s.scale[it % kScaleRing];
-    float top = M;
-    if constexpr (PAGE16) {  // one scale for 16 keys
+    const bool whole = __all_sync(0xffffffffu, see.x <= key0 && see.y >= key0 + kTile);
 #pragma unroll
-      for (int b = 0; b < kTile / 16; ++b) {
-        const float4 y = sc[b * 16];
-        const float by = rf * y.x;
+    for (int c = 0; c < kTile; c += kHalf) {
+      uint32_t x[kHalf];
+      tmem_load32(s_at + c, x);
+      tmem_load32(s_at + c + 32, x + 32);
+      // x = t - M
+      const float ref = M == kNoKey ? 0.0f : M;
+      tmem_loaded();
+      tmem_use<kHalf>(x);
+      if constexpr (PAGE16) {  // one scale for 16 keys
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          x[b * 16 + e] = __float_as_uint(fmaf(__uint_as_float(x[b * 16 + e]), by, y.y));
+        for (int b = 0; b < kHalf; b += 16) {
+          const float4 y = sc[c + b];
+          const float by = rf * y.x, plus = y.y - ref;
+          const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
+#pragma unroll
+          for (int e = b; e < b + 16; e += 2) {
+            const float2 z = unpair(
+                fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by2, plus2));
+            x[e] = __float_as_uint(z.x);
+            x[e + 1] = __float_as_uint(z.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kHalf; ++e) {
+          const float4 y = sc[c + e];
+          x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), rf * y.x, y.y - ref));
+        }
       }
-    } else {
+      if (!whole) {
+        const int lo = see.x - key0 - c, hi = see.y - key0 - c;
 #pragma unroll
-      for (int e = 0; e < kTile; ++e) {
-        const float4 y = sc[e];
-        x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), rf * y.x, y.y));
+        for (int e = 0; e < kHalf; ++e)
+          if (e < lo || e >= hi) x[e] = __float_as_uint(-INFINITY);
       }
-    }
-    const bool whole = see.x <= key0 && see.y >= key0 + kTile;
-    if (!__all_sync(0xffffffffu, whole)) {
-      const int lo = see.x - key0, hi = see.y - key0;
+      float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < kTile; ++e)
-        if (e < lo || e >= hi) x[e] = __float_as_uint(-INFINITY);
-    }
+      for (int e = 0; e < kHalf; e += 4) {
+        top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+        top2 = max3(top2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+      }
+      top = fmaxf(top, top2);
+      const bool passed = M == kNoKey ? top > -INFINITY : top > kLazy;
+      if (__any_sync(0xffffffffu, passed)) {
+        // the reference moves by a whole power of two, so what is rescaled stays exact
+        const float up = passed ? ceilf(top) : 0.0f;
+        const float by = !passed ? 1.0f : M == kNoKey ? 0.0f : ex2(-up);
+        if (passed) M = ref + up;
+        l *= by;
 #pragma unroll
-    for (int e = 0; e < kTile; ++e) top = fmaxf(top, __uint_as_float(x[e]));
-    const bool passed = top > M + kLazy;
-    if (__any_sync(0xffffffffu, passed)) {
-      const float by = passed ? ex2(M - top) : 1.0f;
-      if (passed) M = top;
-      l *= by;
-      if (it > 0) {
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o_at + c, o);
+        for (int e = 0; e < kHalf; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) - up);
+        if (c > 0) {  // this tile's first half is in TMEM already
+          uint32_t p[32];
+          tmem_load32(s_at, p);
           tmem_loaded();
-          tmem_use<32>(o);
+          tmem_use<32>(p);
+          const __half2 by2 = __float2half2_rn(by);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-          tmem_store32(o_at + c, o);
+          for (int e = 0; e < 32; ++e) {
+            const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&p[e]), by2);
+            p[e] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          tmem_store32(s_at, p);
+        }
+        if (it > 0) {
+#pragma unroll 1
+          for (int d = 0; d < D; d += 32) {
+            uint32_t o[32];
+            tmem_load32(o_at + d, o);
+            tmem_loaded();
+            tmem_use<32>(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+            tmem_store32(o_at + d, o);
+          }
         }
       }
-    }
-    uint32_t p[kTile / 2];
-    if constexpr (PAGE16) {
 #pragma unroll
-      for (int b = 0; b < kTile / 16; ++b) {
-        float sum = 0.0f;
+      for (int q = 0; q < kHalf; q += 32) {
+        uint32_t p[16];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = ex2(__uint_as_float(x[b * 16 + e]) - M);
-          const float p1 = ex2(__uint_as_float(x[b * 16 + e + 1]) - M);
-          sum += p0 + p1;
-          p[b * 8 + e / 2] = pack_f16x2(p0, p1);
+        for (int b = q; b < q + 32; b += 16) {
+          uint64_t sum = 0;
+#pragma unroll
+          for (int e = b; e < b + 16; e += 2) {
+            const float p0 = ex2(__uint_as_float(x[e])), p1 = ex2(__uint_as_float(x[e + 1]));
+            if constexpr (PAGE16)
+              sum = add2(sum, pair(p0, p1));
+            else
+              l = fmaf(p1, sc[c + e + 1].z, fmaf(p0, sc[c + e].z, l));
+            p[(e - q) / 2] = pack_f16x2(p0, p1);
+          }
+          if constexpr (PAGE16) {
+            const float2 z = unpair(sum);
+            l = fmaf(z.x + z.y, sc[c + b].z, l);
+          }
         }
-        l = fmaf(sum, sc[b * 16].z, l);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kTile; e += 2) {
-        const float p0 = ex2(__uint_as_float(x[e]) - M);
-        const float p1 = ex2(__uint_as_float(x[e + 1]) - M);
-        l = fmaf(p0, sc[e].z, l);
-        l = fmaf(p1, sc[e + 1].z, l);
-        p[e / 2] = pack_f16x2(p0, p1);
+        tmem_store16(s_at + (c + q) / 2, p);
       }
     }
-    tmem_store32(s_at, p);
-    tmem_store32(s_at + 32, p + 32);
     tmem_stored();
     fence_before();
-    bar_arrive(&s.p_full[t]);
+    warp_arrive(&s.p_full[t]);
   }
 
   if (ok) ok = __all_sync(0xffffffffu, bar_wait(&s.done, 0, &s.gone, a.err));
@@ -565,16 +650,16 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
   const bool two = m0 + kTile < all;
 
   if (threadIdx.x == 0) {
-    bar_init(&s.q_full, 256);
+    bar_init(&s.q_full, 8);  // one arrival a warp
     for (int i = 0; i < 2; ++i) {
-      bar_init(&s.k_full[i], 128);
+      bar_init(&s.k_full[i], 4);
       bar_init(&s.k_empty[i], 1);
-      bar_init(&s.v_full[i], 128);
+      bar_init(&s.v_full[i], 4);
       bar_init(&s.v_empty[i], 1);
       bar_init(&s.s_full[i], 1);
-      bar_init(&s.p_full[i], 128);
+      bar_init(&s.p_full[i], 4);
     }
-    for (int i = 0; i < kScaleRing; ++i) bar_init(&s.scale_full[i], 128);
+    for (int i = 0; i < kScaleRing; ++i) bar_init(&s.scale_full[i], 4);
     bar_init(&s.done, 1);
     s.gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -589,12 +674,12 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
   __syncthreads();
   fence_after();
 
-  // 256 * 184 + 128 * 96 + 128 * 48 = 512 * 128 registers
+  // 256 * 176 + 128 * 112 + 128 * 48 = 512 * 128 registers
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     softmax<D, PAGE16, T>(a, s, rq, h, m0, split, sp, all);
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     loader<D, PAGE16>(a, s, r, h, sp);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
