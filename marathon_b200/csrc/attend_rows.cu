@@ -6,8 +6,8 @@
 //     S_t = Q_t K^T        tcgen05.mma 128 x 128 x D, Q and K f16 in shared memory, S in TMEM
 //     P_t = 2^(t - M)      a thread a row: TMEM -> registers -> f16 -> TMEM, in place of S
 //     O_t += P_t V         tcgen05.mma 128 x D x 128, P from TMEM, V f16 in shared memory
-// Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in,
-// warp 12 issues the matrix products.  While one tile's softmax runs, the other tile's products
+// Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in, warp 12
+// issues the matrix products, warps 13 and 14 look up where the next tiles' keys lie.  While one tile's softmax runs, the other tile's products
 // do, so neither waits for the other in the steady state.
 //
 // e4m3 has no matrix product with f16, so the loaders convert: 16 codes a 16-byte load,
@@ -37,7 +37,7 @@ namespace {
 constexpr int kTile = 128;  // keys of a tile, rows of a row tile
 constexpr int kHalf = 64;   // keys whose scores a softmax thread holds at once
 constexpr int kCta = 512;
-constexpr int kScaleRing = 4;
+constexpr int kRing = 4;  // tiles whose places and scales are held
 constexpr uint32_t kRounds = 1u << 18;  // try_wait rounds of a wait
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -77,6 +77,15 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile 
   *gone = 1;
   flag(err, MSHIFT_EBIT_TIMEOUT);
   return false;
+}
+
+// One lane, and the compiler knows that it is one: what it issues is uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ void commit(uint64_t* b) {
@@ -203,10 +212,10 @@ struct alignas(1024) Smem {
   uint8_t q[2][kBytes];
   uint8_t k[2][kBytes];
   uint8_t v[2][kBytes];
-  float4 scale[kScaleRing][kTile];  // of each key: ks, log2 vs, 1 / vs
-  long long at[2][kTile];           // byte offset of each key in the cache, -1: not read
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[kScaleRing], s_full[2],
-      p_full[2], done;
+  float4 scale[kRing][kTile];  // of each key: ks, log2 vs, 1 / vs
+  long long at[kRing][kTile];  // byte offset of each key in the cache, -1: not read
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], place_full[kRing],
+      place_empty[kRing], s_full[2], p_full[2], done;
   uint32_t tmem;
   int gone;
 };
@@ -222,55 +231,57 @@ struct Span {
   int lo, hi, first, tiles;
 };
 
+// A loader thread has 16 codes of rows tid / 4 + 32 j, at dims 16 (tid % 4) + 64 u: eight
+// neighbouring lanes store to two rows of one swizzle atom, all banks once.
 template <int D>
-__device__ __forceinline__ void load_codes(const uint8_t* base, const long long* at, int part,
-                                           int row0, uint4* w) {
-  constexpr int kPer = D / 16, kStep = 128 / kPer;
-#pragma unroll
-  for (int i = 0; i < kTile / kStep; ++i) {
-    const long long off = at[row0 + i * kStep];
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (off >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(base + off + part * 16));
-  }
-}
-
-template <int D>
-__device__ __forceinline__ void store_f16(uint8_t* tile, int part, int row0, const uint4* w) {
-  constexpr int kPer = D / 16, kStep = 128 / kPer;
-#pragma unroll
-  for (int i = 0; i < kTile / kStep; ++i) {
-    const int row = row0 + i * kStep;
-    uint32_t f[8];
-    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[2 * e] = e4m3x2_to_f16x2((uint16_t)x[e]);
-      f[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(x[e] >> 16));
-    }
-    // eight neighbouring lanes store at once: the lanes of the second 64 dims, whose rows lie
-    // in the same banks, take their two chunks in the other order
-    const bool swap = part >= 4;
-    const uint4 x0 = make_uint4(f[0], f[1], f[2], f[3]), x1 = make_uint4(f[4], f[5], f[6], f[7]);
-    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + swap)) = swap ? x1 : x0;
-    *reinterpret_cast<uint4*>(tile + tile_at<D>(row, 2 * part + !swap)) = swap ? x0 : x1;
-  }
-}
-
-template <int D, bool PAGE16>
-__device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int r, int h, const Span sp) {
+__device__ __forceinline__ void load_codes(const uint8_t* base, const long long* at, uint4* w) {
   const int tid = threadIdx.x - 256;
-  constexpr int kPer = D / 16;
-  const int part = tid % kPer, row0 = tid / kPer;
-  const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
-  const uint8_t* kh = a.k + h * a.head;
-  const uint8_t* vh = a.v + h * a.head;
-  constexpr int kLoads = kTile / (128 / kPer);
-  uint4 kw[kLoads], vw[kLoads];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const long long off = at[tid / 4 + 32 * j];
+    const uint8_t* p = base + off + (tid & 3) * 16;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      w[j * (D / 64) + u] = make_uint4(0, 0, 0, 0);
+      if (off >= 0) w[j * (D / 64) + u] = __ldg(reinterpret_cast<const uint4*>(p + 64 * u));
+    }
+  }
+}
 
-  // Thread t finds key t of a tile, in three steps an iteration apart, so that none waits
-  // for the one before: its block, the block's scales, and their entry in shared memory.
-  auto block_of = [&](int it) -> int {
-    const int key = sp.first + it * kTile + tid;
+template <int D>
+__device__ __forceinline__ void store_f16(uint8_t* tile, const uint4* w) {
+  const int tid = threadIdx.x - 256, row = tid / 4, c = 2 * (tid & 3);
+  uint8_t* at0 = tile + tile_at<D>(row, c);
+  uint8_t* at1 = tile + tile_at<D>(row, c + 1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      const uint4 x = w[j * (D / 64) + u];
+      const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+      uint32_t f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = e4m3x2_to_f16x2((uint16_t)in[e]);
+        f[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(in[e] >> 16));
+      }
+      const int to = j * 32 * 128 + u * kTile * 128;
+      *reinterpret_cast<uint4*>(at0 + to) = make_uint4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<uint4*>(at1 + to) = make_uint4(f[4], f[5], f[6], f[7]);
+    }
+}
+
+// Warps 13 and 14: where the keys of each tile lie and their blocks' scales, two keys a lane.
+// A tile's look-ups are three iterations' work, block, scales and entry, so that none waits for
+// the one before.
+template <int D, bool PAGE16>
+__device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, int h, const Span sp) {
+  const int first = threadIdx.x - 13 * 32;
+  const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
+  const float* ksh = a.ks + h * a.ks_head;
+  const float* vsh = a.vs + h * a.vs_head;
+  auto block_of = [&](int it, int i) -> int {
+    const int key = sp.first + it * kTile + first + 64 * i;
     // PAGE16 reads the scales of 16 keys at the first of them, which may itself be outside
     if (it >= sp.tiles ||
         (PAGE16 ? (key | 15) < sp.lo || (key & ~15) >= sp.hi : key < sp.lo || key >= sp.hi))
@@ -280,59 +291,78 @@ __device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int r, i
     flag(a.err, MSHIFT_EBIT_SLOT);
     return -1;
   };
-  auto scales_of = [&](int b, float& ks, float& vs) {
-    if (b < 0) return;
-    ks = a.ks[b * a.ks_blk + h * a.ks_head];
-    vs = a.vs[b * a.vs_blk + h * a.vs_head];
-  };
-  auto publish = [&](int it, int b, float ks, float vs) {
-    const int key = sp.first + it * kTile + tid;
-    vs = fmaxf(vs, kScaleFloor);
-    s.at[it & 1][tid] =
-        b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + key % a.bs * a.off : -1ll;
-    s.scale[it % kScaleRing][tid] = b >= 0 ? make_float4(ks, __log2f(vs), __frcp_rn(vs), 0.0f)
-                                           : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-    warp_arrive(&s.scale_full[it % kScaleRing]);
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-  };
-
-  float ks1 = 0.0f, vs1 = 0.0f;
-  int b1 = block_of(0), b2 = block_of(1);
-  scales_of(b1, ks1, vs1);
-  publish(0, b1, ks1, vs1);
-  load_codes<D>(kh, s.at[0], part, row0, kw);
-  load_codes<D>(vh, s.at[0], part, row0, vw);
-  b1 = b2;
-  scales_of(b1, ks1, vs1);
-  b2 = block_of(2);
-  bool ok = true;
+  int b1[2], b2[2];
+  float ks[2], vs[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    b1[i] = block_of(0, i);
+    b2[i] = block_of(1, i);
+    ks[i] = vs[i] = 0.0f;
+    if (b1[i] >= 0) {
+      ks[i] = ksh[b1[i] * a.ks_blk];
+      vs[i] = vsh[b1[i] * a.vs_blk];
+    }
+  }
   for (int it = 0; it < sp.tiles; ++it) {
+    const int ring = it % kRing;
+    if (!__all_sync(0xffffffffu,
+                    bar_wait(&s.place_empty[ring], ((it / kRing) & 1) ^ 1, &s.gone, a.err)))
+      return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = first + 64 * i, key = sp.first + it * kTile + at, b = b1[i];
+      const float v = fmaxf(vs[i], kScaleFloor);
+      s.at[ring][at] = b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + key % a.bs * a.off : -1ll;
+      s.scale[ring][at] = b >= 0 ? make_float4(ks[i], __log2f(v), __frcp_rn(v), 0.0f)
+                                 : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    }
+    warp_arrive(&s.place_full[ring]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      b1[i] = b2[i];
+      if (b1[i] >= 0) {
+        ks[i] = ksh[b1[i] * a.ks_blk];
+        vs[i] = vsh[b1[i] * a.vs_blk];
+      }
+      b2[i] = block_of(it + 2, i);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int h, int tiles) {
+  const uint8_t* kh = a.k + h * a.head;
+  const uint8_t* vh = a.v + h * a.head;
+  uint4 kw[D / 16], vw[D / 16];
+  auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  auto placed = [&](int it) {
+    return all(bar_wait(&s.place_full[it % kRing], (it / kRing) & 1, &s.gone, a.err));
+  };
+  if (!placed(0)) return;
+  load_codes<D>(kh, s.at[0], kw);
+  load_codes<D>(vh, s.at[0], vw);
+  warp_arrive(&s.place_empty[0]);
+  for (int it = 0; it < tiles; ++it) {
     const int st = it & 1;
     const uint32_t free = ((it >> 1) & 1) ^ 1;
-    const bool more = it + 1 < sp.tiles;
-    ok = ok && bar_wait(&s.k_empty[st], free, &s.gone, a.err);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
-      store_f16<D>(s.k[st], part, row0, kw);
-      fence_smem();
-      warp_arrive(&s.k_full[st]);
-    }
-    // every loader meets here even after a wait ran out, or the others would hang
+    const bool more = it + 1 < tiles;
+    // the codes of a tile are loaded an iteration before they are converted
+    if (!all(bar_wait(&s.k_empty[st], free, &s.gone, a.err))) return;
+    store_f16<D>(s.k[st], kw);
+    fence_smem();
+    warp_arrive(&s.k_full[st]);
     if (more) {
-      publish(it + 1, b1, ks1, vs1);
-      load_codes<D>(kh, s.at[(it + 1) & 1], part, row0, kw);
-      b1 = b2;
-      scales_of(b1, ks1, vs1);
-      b2 = block_of(it + 3);
+      if (!placed(it + 1)) return;
+      load_codes<D>(kh, s.at[(it + 1) % kRing], kw);
     }
-    ok = ok && bar_wait(&s.v_empty[st], free, &s.gone, a.err);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
-      store_f16<D>(s.v[st], part, row0, vw);
-      fence_smem();
-      warp_arrive(&s.v_full[st]);
+    if (!all(bar_wait(&s.v_empty[st], free, &s.gone, a.err))) return;
+    store_f16<D>(s.v[st], vw);
+    fence_smem();
+    warp_arrive(&s.v_full[st]);
+    if (more) {
+      load_codes<D>(vh, s.at[(it + 1) % kRing], vw);
+      warp_arrive(&s.place_empty[(it + 1) % kRing]);
     }
-    if (more) load_codes<D>(vh, s.at[(it + 1) & 1], part, row0, vw);
   }
 }
 
@@ -442,12 +472,12 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   bool ok = true;
   for (int it = 0; it < sp.tiles; ++it) {
     const int key0 = sp.first + it * kTile;
-    ok = bar_wait(&s.scale_full[it % kScaleRing], (it / kScaleRing) & 1, &s.gone, a.err);
+    ok = bar_wait(&s.place_full[it % kRing], (it / kRing) & 1, &s.gone, a.err);
     ok = ok && bar_wait(&s.s_full[t], it & 1, &s.gone, a.err);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     fence_after();
-    const float4* sc = s.scale[it % kScaleRing];
+    const float4* sc = s.scale[it % kRing];
     const bool whole = __all_sync(0xffffffffu, see.x <= key0 && see.y >= key0 + kTile);
 #pragma unroll
     for (int c = 0; c < kTile; c += kHalf) {
@@ -553,6 +583,7 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
     tmem_stored();
     fence_before();
     warp_arrive(&s.p_full[t]);
+    warp_arrive(&s.place_empty[it % kRing]);
   }
 
   if (ok) ok = __all_sync(0xffffffffu, bar_wait(&s.done, 0, &s.gone, a.err));
@@ -659,7 +690,10 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
       bar_init(&s.s_full[i], 1);
       bar_init(&s.p_full[i], 4);
     }
-    for (int i = 0; i < kScaleRing; ++i) bar_init(&s.scale_full[i], 4);
+    for (int i = 0; i < kRing; ++i) {
+      bar_init(&s.place_full[i], 2);
+      bar_init(&s.place_empty[i], two ? 12 : 8);  // softmax warps of live tiles, loaders
+    }
     bar_init(&s.done, 1);
     s.gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -680,17 +714,19 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
     softmax<D, PAGE16, T>(a, s, rq, h, m0, split, sp, all);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    loader<D, PAGE16>(a, s, r, h, sp);
+    loader<D>(a, s, h, sp.tiles);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 12) {
-      if ((threadIdx.x & 31) == 0) {
+      if (elect_one()) {
         issuer<D>(a, s, sp.tiles, two);
         // after a wait that ran out nobody else waits for the products
         for (uint32_t i = 0; i < kRounds && !bar_try(&s.done, 0); ++i) {
         }
       }
       __syncwarp();
+    } else if (warp < 15) {
+      finder<D, PAGE16>(a, s, r, h, sp);
     }
   }
   fence_before();
