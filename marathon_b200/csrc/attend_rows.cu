@@ -16,11 +16,10 @@
 // contraction (K-major), V with its tokens (MN-major), so no tile is transposed.
 // A code is converted once for 256 rows.
 //
-// TMEM columns: S (then P) of tile 0 at 0, of tile 1 at 128, O of tile 0 at 256, of tile 1 at 256 + D.
-// O is rescaled in place when a row's maximum passes its reference by 2^8, which is rare after
-// the first tiles; S_t of a key tile is complete only after the product P_t V of
-// the one before (one thread issues them in that order and the commit covers both),
-// so the rescaling thread needs no further barrier.
+// The keys of a tile are taken in halves of 64, each with its own S (then P) columns: while the
+// softmax has one half, the other's products run.  TMEM columns: S of row tile t, half b at
+// 128 t + 64 b, O of tile t at 256 + D t.  O is rescaled in place when a row's maximum passes its
+// reference by 2^8, after the product before has completed; that is rare after the first tiles.
 //
 // Registers: 512 threads are launched with 128 each; the softmax warps take 176
 // (64 scores of a row at once), the loaders 112 (two tiles' codes in flight) and the rest 48,
@@ -215,7 +214,7 @@ struct alignas(1024) Smem {
   float4 scale[kRing][kTile];  // of each key: ks, log2 vs, 1 / vs
   long long at[kRing][kTile];  // byte offset of each key in the cache, -1: not read
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], place_full[kRing],
-      place_empty[kRing], s_full[2], p_full[2], done;
+      place_empty[kRing], s_full[2][2], p_full[2][2], o_done[2], done;
   uint32_t tmem;
   int gone;
 };
@@ -368,47 +367,56 @@ __device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int h, i
 
 template <int D>
 __device__ __forceinline__ void issuer(const AttendArgs& a, Smem<D>& s, int tiles, bool two) {
-  constexpr uint32_t kScore = instruction(kTile, false), kValue = instruction(D, true);
+  constexpr uint32_t kScore = instruction(kHalf, false), kValue = instruction(D, true);
   const uint32_t tmem = s.tmem;
   const uint32_t q0 = smem_u32(s.q[0]), k0 = smem_u32(s.k[0]), v0 = smem_u32(s.v[0]);
-  auto scores = [&](int t, int st) {
+  // half n of the keys: rows 64 (n % 2) of stage (n / 2) % 2, buffer n % 2
+  auto scores = [&](int t, int n) {
+    const uint64_t qd = descriptor(q0 + t * Smem<D>::kBytes, 16);
+    const uint64_t kd = descriptor(k0 + ((n >> 1) & 1) * Smem<D>::kBytes + (n & 1) * (kHalf * 128), 16);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {  // 16 dims: 32 bytes of a 128-byte row
-      const uint32_t in = (d >> 2) * (kTile * 128) + (d & 3) * 32;
-      mma_smem(tmem + t * kTile, descriptor(q0 + t * Smem<D>::kBytes + in, 16),
-               descriptor(k0 + st * Smem<D>::kBytes + in, 16), kScore, d > 0);
+      const uint32_t in = ((d >> 2) * (kTile * 128) + (d & 3) * 32) >> 4;
+      mma_smem(tmem + t * kTile + (n & 1) * kHalf, qd + in, kd + in, kScore, d > 0);
     }
-    commit(&s.s_full[t]);
+    commit(&s.s_full[t][n & 1]);
   };
+  auto values = [&](int t, int n) {
+    const uint64_t vd =
+        descriptor(v0 + ((n >> 1) & 1) * Smem<D>::kBytes + (n & 1) * (kHalf * 128), kTile * 128);
+#pragma unroll
+    for (int k = 0; k < kHalf / 16; ++k)  // 16 keys: two groups of 8 rows
+      mma_tmem(tmem + 256 + t * D, tmem + t * kTile + (n & 1) * kHalf + k * 8, vd + (k * 2048 >> 4),
+               kValue, n > 0 || k > 0);
+    commit(&s.o_done[t]);
+  };
+  const int row_tiles = two ? 2 : 1, halves = 2 * tiles;
   bool ok = bar_wait(&s.q_full, 0, &s.gone, a.err) && bar_wait(&s.k_full[0], 0, &s.gone, a.err);
   fence_after();
   if (ok) {
-    scores(0, 0);
-    if (two) scores(1, 0);
+    for (int n = 0; n < 2; ++n)
+      for (int t = 0; t < row_tiles; ++t) scores(t, n);
     commit(&s.k_empty[0]);
   }
-  for (int it = 0; ok && it < tiles; ++it) {
-    const int st = it & 1, nx = (it + 1) & 1;
-    ok = bar_wait(&s.v_full[st], (it >> 1) & 1, &s.gone, a.err);
-    for (int t = 0; ok && t < (two ? 2 : 1); ++t) {
-      ok = bar_wait(&s.p_full[t], it & 1, &s.gone, a.err);
+  for (int n = 0; ok && n < halves; ++n) {
+    const int it = n >> 1, st = it & 1, b = n & 1;
+    if (b == 0) ok = bar_wait(&s.v_full[st], it & 2 ? 1 : 0, &s.gone, a.err);
+    for (int t = 0; ok && t < row_tiles; ++t) {
+      ok = bar_wait(&s.p_full[t][b], it & 1, &s.gone, a.err);
       if (!ok) break;
       fence_after();
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)  // 16 keys: two groups of 8 rows
-        mma_tmem(tmem + 256 + t * D, tmem + t * kTile + k * 8,
-                 descriptor(v0 + st * Smem<D>::kBytes + k * 2048, kTile * 128), kValue,
-                 it > 0 || k > 0);
-      if (it + 1 < tiles) {
-        if (t == 0) ok = bar_wait(&s.k_full[nx], ((it + 1) >> 1) & 1, &s.gone, a.err);
+      values(t, n);
+      if (n + 2 < halves) {
+        if (b == 0 && t == 0)
+          ok = bar_wait(&s.k_full[st ^ 1], ((it + 1) >> 1) & 1, &s.gone, a.err);
         if (!ok) break;
-        fence_after();
-        scores(t, nx);
+        scores(t, n + 2);
       }
     }
-    if (!ok) break;
-    commit(&s.v_empty[st]);
-    if (it + 1 < tiles) commit(&s.k_empty[nx]);
+    if (ok && b == 1) {
+      commit(&s.v_empty[st]);
+      if (n + 2 < halves) commit(&s.k_empty[st ^ 1]);
+    }
   }
   // also after a wait ran out: what was issued completes before TMEM is freed
   commit(&s.done);
@@ -470,120 +478,106 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   const uint32_t s_at = s.tmem + lanes + t * kTile, o_at = s.tmem + lanes + 256 + t * D;
   float M = kNoKey, l = 0.0f;
   bool ok = true;
-  for (int it = 0; it < sp.tiles; ++it) {
-    const int key0 = sp.first + it * kTile;
-    ok = bar_wait(&s.place_full[it % kRing], (it / kRing) & 1, &s.gone, a.err);
-    ok = ok && bar_wait(&s.s_full[t], it & 1, &s.gone, a.err);
+  for (int n = 0; n < 2 * sp.tiles; ++n) {
+    const int it = n >> 1, b = n & 1, key0 = sp.first + n * kHalf;
+    if (b == 0) ok = bar_wait(&s.place_full[it % kRing], (it / kRing) & 1, &s.gone, a.err);
+    ok = ok && bar_wait(&s.s_full[t][b], it & 1, &s.gone, a.err);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     fence_after();
-    const float4* sc = s.scale[it % kRing];
-    const bool whole = __all_sync(0xffffffffu, see.x <= key0 && see.y >= key0 + kTile);
+    const float4* sc = s.scale[it % kRing] + b * kHalf;
+    const uint32_t sb_at = s_at + b * kHalf;
+    uint32_t x[kHalf];
+    tmem_load32(sb_at, x);
+    tmem_load32(sb_at + 32, x + 32);
+    // x = t - M
+    const float ref = M == kNoKey ? 0.0f : M;
+    tmem_loaded();
+    tmem_use<kHalf>(x);
+    if constexpr (PAGE16) {  // one scale for 16 keys
 #pragma unroll
-    for (int c = 0; c < kTile; c += kHalf) {
-      uint32_t x[kHalf];
-      tmem_load32(s_at + c, x);
-      tmem_load32(s_at + c + 32, x + 32);
-      // x = t - M
-      const float ref = M == kNoKey ? 0.0f : M;
-      tmem_loaded();
-      tmem_use<kHalf>(x);
-      if constexpr (PAGE16) {  // one scale for 16 keys
+      for (int c = 0; c < kHalf; c += 16) {
+        const float4 y = sc[c];
+        const float by = rf * y.x, plus = y.y - ref;
+        const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
 #pragma unroll
-        for (int b = 0; b < kHalf; b += 16) {
-          const float4 y = sc[c + b];
-          const float by = rf * y.x, plus = y.y - ref;
-          const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
-#pragma unroll
-          for (int e = b; e < b + 16; e += 2) {
-            const float2 z = unpair(
-                fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by2, plus2));
-            x[e] = __float_as_uint(z.x);
-            x[e + 1] = __float_as_uint(z.y);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kHalf; ++e) {
-          const float4 y = sc[c + e];
-          x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), rf * y.x, y.y - ref));
+        for (int e = c; e < c + 16; e += 2) {
+          const float2 z =
+              unpair(fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by2, plus2));
+          x[e] = __float_as_uint(z.x);
+          x[e + 1] = __float_as_uint(z.y);
         }
       }
-      if (!whole) {
-        const int lo = see.x - key0 - c, hi = see.y - key0 - c;
+    } else {
 #pragma unroll
-        for (int e = 0; e < kHalf; ++e)
-          if (e < lo || e >= hi) x[e] = __float_as_uint(-INFINITY);
+      for (int e = 0; e < kHalf; ++e) {
+        const float4 y = sc[e];
+        x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), rf * y.x, y.y - ref));
       }
-      float top = -INFINITY, top2 = -INFINITY;
+    }
+    if (!__all_sync(0xffffffffu, see.x <= key0 && see.y >= key0 + kHalf)) {
+      const int lo = see.x - key0, hi = see.y - key0;
 #pragma unroll
-      for (int e = 0; e < kHalf; e += 4) {
-        top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-        top2 = max3(top2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-      }
-      top = fmaxf(top, top2);
-      const bool passed = M == kNoKey ? top > -INFINITY : top > kLazy;
-      if (__any_sync(0xffffffffu, passed)) {
-        // the reference moves by a whole power of two, so what is rescaled stays exact
-        const float up = passed ? ceilf(top) : 0.0f;
-        const float by = !passed ? 1.0f : M == kNoKey ? 0.0f : ex2(-up);
-        if (passed) M = ref + up;
-        l *= by;
+      for (int e = 0; e < kHalf; ++e)
+        if (e < lo || e >= hi) x[e] = __float_as_uint(-INFINITY);
+    }
+    float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < kHalf; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) - up);
-        if (c > 0) {  // this tile's first half is in TMEM already
-          uint32_t p[32];
-          tmem_load32(s_at, p);
-          tmem_loaded();
-          tmem_use<32>(p);
-          const __half2 by2 = __float2half2_rn(by);
+    for (int e = 0; e < kHalf; e += 4) {
+      top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+      top2 = max3(top2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+    }
+    top = fmaxf(top, top2);
+    const bool passed = M == kNoKey ? top > -INFINITY : top > kLazy;
+    if (__any_sync(0xffffffffu, passed)) {
+      const float up = passed ? top : 0.0f;
+      const float by = !passed ? 1.0f : M == kNoKey ? 0.0f : ex2(-up);
+      if (passed) M = ref + up;
+      l *= by;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&p[e]), by2);
-            p[e] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          tmem_store32(s_at, p);
-        }
-        if (it > 0) {
+      for (int e = 0; e < kHalf; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) - up);
+      if (n > 0) {  // O holds every half before this one once the last product is done
+        ok = __all_sync(0xffffffffu, bar_wait(&s.o_done[t], (n - 1) & 1, &s.gone, a.err));
+        if (!ok) break;
+        fence_after();
 #pragma unroll 1
-          for (int d = 0; d < D; d += 32) {
-            uint32_t o[32];
-            tmem_load32(o_at + d, o);
-            tmem_loaded();
-            tmem_use<32>(o);
+        for (int d = 0; d < D; d += 32) {
+          uint32_t o[32];
+          tmem_load32(o_at + d, o);
+          tmem_loaded();
+          tmem_use<32>(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-            tmem_store32(o_at + d, o);
-          }
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+          tmem_store32(o_at + d, o);
         }
       }
+    }
 #pragma unroll
-      for (int q = 0; q < kHalf; q += 32) {
-        uint32_t p[16];
+    for (int q = 0; q < kHalf; q += 32) {
+      uint32_t p[16];
 #pragma unroll
-        for (int b = q; b < q + 32; b += 16) {
-          uint64_t sum = 0;
+      for (int c = q; c < q + 32; c += 16) {
+        uint64_t sum = 0;
 #pragma unroll
-          for (int e = b; e < b + 16; e += 2) {
-            const float p0 = ex2(__uint_as_float(x[e])), p1 = ex2(__uint_as_float(x[e + 1]));
-            if constexpr (PAGE16)
-              sum = add2(sum, pair(p0, p1));
-            else
-              l = fmaf(p1, sc[c + e + 1].z, fmaf(p0, sc[c + e].z, l));
-            p[(e - q) / 2] = pack_f16x2(p0, p1);
-          }
-          if constexpr (PAGE16) {
-            const float2 z = unpair(sum);
-            l = fmaf(z.x + z.y, sc[c + b].z, l);
-          }
+        for (int e = c; e < c + 16; e += 2) {
+          const float p0 = ex2(__uint_as_float(x[e])), p1 = ex2(__uint_as_float(x[e + 1]));
+          if constexpr (PAGE16)
+            sum = add2(sum, pair(p0, p1));
+          else
+            l = fmaf(p1, sc[e + 1].z, fmaf(p0, sc[e].z, l));
+          p[(e - q) / 2] = pack_f16x2(p0, p1);
         }
-        tmem_store16(s_at + (c + q) / 2, p);
+        if constexpr (PAGE16) {
+          const float2 z = unpair(sum);
+          l = fmaf(z.x + z.y, sc[c].z, l);
+        }
       }
+      tmem_store16(sb_at + q / 2, p);
     }
     tmem_stored();
     fence_before();
-    warp_arrive(&s.p_full[t]);
-    warp_arrive(&s.place_empty[it % kRing]);
+    warp_arrive(&s.p_full[t][b]);
+    if (b == 1) warp_arrive(&s.place_empty[it % kRing]);
   }
 
   if (ok) ok = __all_sync(0xffffffffu, bar_wait(&s.done, 0, &s.gone, a.err));
@@ -687,8 +681,11 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
       bar_init(&s.k_empty[i], 1);
       bar_init(&s.v_full[i], 4);
       bar_init(&s.v_empty[i], 1);
-      bar_init(&s.s_full[i], 1);
-      bar_init(&s.p_full[i], 4);
+      for (int b = 0; b < 2; ++b) {
+        bar_init(&s.s_full[i][b], 1);
+        bar_init(&s.p_full[i][b], 4);
+      }
+      bar_init(&s.o_done[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
       bar_init(&s.place_full[i], 2);
