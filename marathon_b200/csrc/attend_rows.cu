@@ -215,6 +215,7 @@ struct alignas(1024) Smem {
   long long at[kRing][kTile];  // byte offset of each key in the cache, -1: not read
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], place_full[kRing],
       place_empty[kRing], s_full[2][2], p_full[2][2], o_done[2], done;
+  float up[2][kTile];  // of each row: what its scores are multiplied with, log2 e among it
   uint32_t tmem;
   int gone;
 };
@@ -422,6 +423,12 @@ __device__ __forceinline__ void issuer(const AttendArgs& a, Smem<D>& s, int tile
   commit(&s.done);
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const float f[2] = {lo, hi};
+  return Elem<T>::pack(f);
+}
+
 // Rows 32 * (warp % 4) + lane of tile t.
 template <int D, bool PAGE16, typename T>
 __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const Request& rq, int h,
@@ -432,46 +439,54 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   const bool live = m < all;
   const int64_t tok = rq.q0 + (live ? m / a.group : 0);
   const int hq = h * a.group + (live ? m % a.group : 0);
-  int2 see = live ? seen(a, rq, rq.start + m / a.group) : make_int2(0, 0);
+  const int mine = all - (m - lane);  // the warp's live rows, or more than 32
+  int2 see = live ? seen(a, rq, rq.start + (tok - rq.q0)) : make_int2(0, 0);
   see.x = max(see.x, sp.lo);
   see.y = min(see.y, sp.hi);
 
-  // the query row: f16 after a power of two
-  float rf = a.scale_log2;
-  {
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.q_tok +
-                                                      hq * a.q_head);
-    float top = 0.0f;
-    for (int c = 0; c < D / 8; ++c) {
-      const uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+  // the warp's query rows, a row on D / 8 lanes: f16 after a power of two
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a warp-wide load
+  constexpr int kAhead = 8;                           // loads in flight
+  const int64_t q_row = tok * a.q_tok + hq * a.q_head;  // of this lane's row; others' by shuffle
+#pragma unroll 1
+  for (int i0 = 0; i0 < kLanes; i0 += kAhead) {
+    uint4 w[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int from = (i0 + i) * kRows + lane / kLanes;
+      const int64_t at = __shfl_sync(0xffffffffu, q_row, from);
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (from < mine)
+        w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + lane % kLanes);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = (warp & 3) * 32 + (i0 + i) * kRows + lane / kLanes;
       float f[8];
-      Elem<T>::unpack(w.x, f);
-      Elem<T>::unpack(w.y, f + 2);
-      Elem<T>::unpack(w.z, f + 4);
-      Elem<T>::unpack(w.w, f + 6);
+      Elem<T>::unpack(w[i].x, f);
+      Elem<T>::unpack(w[i].y, f + 2);
+      Elem<T>::unpack(w[i].z, f + 4);
+      Elem<T>::unpack(w[i].w, f + 6);
+      float top = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-    }
-    int e2 = (int)(__float_as_uint(top) >> 23) - 127;
-    if (e2 < -126 || e2 > 126) e2 = 0;
-    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-    rf *= __uint_as_float((uint32_t)(127 + e2) << 23);
-    for (int c = 0; c < D / 8; ++c) {
-      const uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
-      float f[8];
-      Elem<T>::unpack(w.x, f);
-      Elem<T>::unpack(w.y, f + 2);
-      Elem<T>::unpack(w.z, f + 4);
-      Elem<T>::unpack(w.w, f + 6);
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+      if (e2 < -126 || e2 > 126) e2 = 0;
+      const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= down;
-      *reinterpret_cast<uint4*>(s.q[t] + tile_at<D>(row, c)) =
+      *reinterpret_cast<uint4*>(s.q[t] + tile_at<D>(at, lane % kLanes)) =
           make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]),
                      pack_f16x2(f[6], f[7]));
+      if (lane % kLanes == 0)
+        s.up[t][at] = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
     }
-    fence_smem();
-    warp_arrive(&s.q_full);
   }
+  fence_smem();
+  warp_arrive(&s.q_full);
+  const float rf = s.up[t][row];  // its own warp's
   if (m0 + t * kTile >= all) return;  // a tile without rows
 
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -586,36 +601,47 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   const bool any = M > kNoKey;
   const float by = any ? 1.0f / l : 0.0f;
   const int64_t part = (tok * a.hq + hq) * a.rsplit + split;
+  if (live && a.rsplit > 1)
+    a.rpart_ml[part] = make_float2(M, l);
+  else if (live && a.lse != nullptr)
+    a.lse[tok * a.hq + hq] = any ? (M + log2f(l)) * kLn2 : -INFINITY;
+  // Rows go through shared memory (K's and V's, done with), so that whole rows are written: 32 rows of
+  // D words a warp, 16-byte chunks swizzled by row.
+  float4* stage = reinterpret_cast<float4*>((t ? s.v : s.k)[0]) + (warp & 3) * (32 * D / 4);
 #pragma unroll
   for (int c = 0; c < D; c += 32) {
     uint32_t o[32];
     tmem_load32(o_at + c, o);
     tmem_loaded();
     tmem_use<32>(o);
-    if (!live) continue;
-    if (a.rsplit > 1) {
-      float4* dst = reinterpret_cast<float4*>(a.rpart_o + part * D + c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                             __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-    } else {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_tok + hq * a.o_head + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = any ? __uint_as_float(o[8 * e + i]) * by : 0.0f;
-        dst[e] = make_uint4(Elem<T>::pack(f), Elem<T>::pack(f + 2), Elem<T>::pack(f + 4),
-                            Elem<T>::pack(f + 6));
-      }
-    }
+    for (int e = 0; e < 8; ++e)
+      stage[lane * (D / 4) + ((c / 4 + e) ^ (lane & 7))] =
+          make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                      __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
   }
-  if (!live) return;
-  if (a.rsplit > 1)
-    a.rpart_ml[part] = make_float2(M, l);
-  else if (a.lse != nullptr)
-    a.lse[tok * a.hq + hq] = any ? (M + log2f(l)) * kLn2 : -INFINITY;
+  __syncwarp();
+  constexpr int kLanesOut = D / 4;  // lanes of a row of float4
+  const bool parts = a.rsplit > 1;
+  const int64_t o_row = parts ? part * D : tok * a.o_tok + hq * a.o_head;
+  const float mul = !any ? 0.0f : parts ? 1.0f : by;
+  T* out = static_cast<T*>(a.out) + lane % kLanesOut * 4;
+  float* part_o = a.rpart_o + lane % kLanesOut * 4;
+#pragma unroll 4
+  for (int i = 0; i < kLanesOut; ++i) {
+    const int from = i * (32 / kLanesOut) + lane / kLanesOut;
+    float4 y = stage[from * kLanesOut + (lane % kLanesOut ^ (from & 7))];
+    const int64_t to = __shfl_sync(0xffffffffu, o_row, from);
+    const float scale = __shfl_sync(0xffffffffu, mul, from);
+    if (from >= mine) continue;
+    // a row without keys is zeros, whatever the values beside it were
+    y = scale == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                      : make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
+    if (parts)
+      *reinterpret_cast<float4*>(part_o + to) = y;
+    else
+      *reinterpret_cast<uint2*>(out + to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+  }
 }
 
 // Rows without a key in this CTA's span: an empty part, or zeros.
