@@ -6,8 +6,8 @@
 //     S_t = Q_t K^T        tcgen05.mma 128 x 128 x D, Q and K f16 in shared memory, S in TMEM
 //     P_t = 2^(t - M)      a thread a row: TMEM -> registers -> f16 -> TMEM, in place of S
 //     O_t += P_t V         tcgen05.mma 128 x D x 128, P from TMEM, V f16 in shared memory
-// Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in, warp 12
-// issues the matrix products, warps 13 and 14 look up where the next tiles' keys lie.  While one tile's softmax runs, the other tile's products
+// Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in, warps 12 and 13
+// issue the products of tile 0 and 1, warps 14 and 15 look up where the next tiles' keys lie.  While one tile's softmax runs, the other tile's products
 // do, so neither waits for the other in the steady state.
 //
 // e4m3 has no matrix product with f16, so the loaders convert: 16 codes a 16-byte load,
@@ -69,6 +69,7 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* gone,
                                          uint32_t* err) {
   if (bar_try(b, parity)) return true;
+#pragma unroll 1
   for (uint32_t i = 0; i < kRounds; ++i) {
     if (bar_try(b, parity)) return true;
     if (*gone) return false;
@@ -271,12 +272,12 @@ __device__ __forceinline__ void store_f16(uint8_t* tile, const uint4* w) {
     }
 }
 
-// Warps 13 and 14: where the keys of each tile lie and their blocks' scales, two keys a lane.
+// Warps 14 and 15: where the keys of each tile lie and their blocks' scales, two keys a lane.
 // A tile's look-ups are three iterations' work, block, scales and entry, so that none waits for
 // the one before.
 template <int D, bool PAGE16>
 __device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, int h, const Span sp) {
-  const int first = threadIdx.x - 13 * 32;
+  const int first = threadIdx.x - 14 * 32;
   const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
   const float* ksh = a.ks + h * a.ks_head;
   const float* vsh = a.vs + h * a.vs_head;
@@ -303,6 +304,7 @@ __device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, i
       vs[i] = vsh[b1[i] * a.vs_blk];
     }
   }
+#pragma unroll 1
   for (int it = 0; it < sp.tiles; ++it) {
     const int ring = it % kRing;
     if (!__all_sync(0xffffffffu,
@@ -342,6 +344,7 @@ __device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int h, i
   load_codes<D>(kh, s.at[0], kw);
   load_codes<D>(vh, s.at[0], vw);
   warp_arrive(&s.place_empty[0]);
+#pragma unroll 1
   for (int it = 0; it < tiles; ++it) {
     const int st = it & 1;
     const uint32_t free = ((it >> 1) & 1) ^ 1;
@@ -366,57 +369,59 @@ __device__ __forceinline__ void loader(const AttendArgs& a, Smem<D>& s, int h, i
   }
 }
 
+// The products of row tile t, issued by one lane.  Each tile has a warp of its own: the products wait in
+// a queue and their operands' registers with them, so a warp that issues cannot prepare the next ones
+// until they start; two warps keep the tensor core supplied between them.
 template <int D>
-__device__ __forceinline__ void issuer(const AttendArgs& a, Smem<D>& s, int tiles, bool two) {
+__device__ __forceinline__ void issuer(const AttendArgs& a, Smem<D>& s, int tiles, int t) {
   constexpr uint32_t kScore = instruction(kHalf, false), kValue = instruction(D, true);
-  const uint32_t tmem = s.tmem;
-  const uint32_t q0 = smem_u32(s.q[0]), k0 = smem_u32(s.k[0]), v0 = smem_u32(s.v[0]);
-  // half n of the keys: rows 64 (n % 2) of stage (n / 2) % 2, buffer n % 2
-  auto scores = [&](int t, int n) {
-    const uint64_t qd = descriptor(q0 + t * Smem<D>::kBytes, 16);
-    const uint64_t kd = descriptor(k0 + ((n >> 1) & 1) * Smem<D>::kBytes + (n & 1) * (kHalf * 128), 16);
+  const uint32_t s_at = s.tmem + t * kTile, o_at = s.tmem + 256 + t * D;
+  const uint64_t q_desc = descriptor(smem_u32(s.q[t]), 16), k_desc = descriptor(smem_u32(s.k[0]), 16),
+                 v_desc = descriptor(smem_u32(s.v[0]), kTile * 128);
+  // half n of the keys: rows 64 (n % 2) of stage (n / 2) % 2, columns 64 (n % 2)
+  auto stage = [](int n) -> uint32_t {
+    return (((n >> 1) & 1) * Smem<D>::kBytes + (n & 1) * (kHalf * 128)) >> 4;
+  };
+  auto scores = [&](int n) {
+    const uint64_t kd = k_desc + stage(n);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {  // 16 dims: 32 bytes of a 128-byte row
       const uint32_t in = ((d >> 2) * (kTile * 128) + (d & 3) * 32) >> 4;
-      mma_smem(tmem + t * kTile + (n & 1) * kHalf, qd + in, kd + in, kScore, d > 0);
+      mma_smem(s_at + (n & 1) * kHalf, q_desc + in, kd + in, kScore, d > 0);
     }
     commit(&s.s_full[t][n & 1]);
   };
-  auto values = [&](int t, int n) {
-    const uint64_t vd =
-        descriptor(v0 + ((n >> 1) & 1) * Smem<D>::kBytes + (n & 1) * (kHalf * 128), kTile * 128);
+  auto values = [&](int n) {
+    const uint64_t vd = v_desc + stage(n);
 #pragma unroll
     for (int k = 0; k < kHalf / 16; ++k)  // 16 keys: two groups of 8 rows
-      mma_tmem(tmem + 256 + t * D, tmem + t * kTile + (n & 1) * kHalf + k * 8, vd + (k * 2048 >> 4),
-               kValue, n > 0 || k > 0);
+      mma_tmem(o_at, s_at + (n & 1) * kHalf + k * 8, vd + (k * 2048 >> 4), kValue, n > 0 || k > 0);
     commit(&s.o_done[t]);
   };
-  const int row_tiles = two ? 2 : 1, halves = 2 * tiles;
   bool ok = bar_wait(&s.q_full, 0, &s.gone, a.err) && bar_wait(&s.k_full[0], 0, &s.gone, a.err);
   fence_after();
   if (ok) {
-    for (int n = 0; n < 2; ++n)
-      for (int t = 0; t < row_tiles; ++t) scores(t, n);
+    scores(0);
+    scores(1);
     commit(&s.k_empty[0]);
   }
-  for (int n = 0; ok && n < halves; ++n) {
-    const int it = n >> 1, st = it & 1, b = n & 1;
-    if (b == 0) ok = bar_wait(&s.v_full[st], it & 2 ? 1 : 0, &s.gone, a.err);
-    for (int t = 0; ok && t < row_tiles; ++t) {
-      ok = bar_wait(&s.p_full[t][b], it & 1, &s.gone, a.err);
+#pragma unroll 1
+  for (int it = 0; ok && it < tiles; ++it) {
+    const int st = it & 1;
+    const bool more = it + 1 < tiles;
+    ok = bar_wait(&s.v_full[st], (it >> 1) & 1, &s.gone, a.err);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      ok = ok && bar_wait(&s.p_full[t][b], it & 1, &s.gone, a.err);
       if (!ok) break;
       fence_after();
-      values(t, n);
-      if (n + 2 < halves) {
-        if (b == 0 && t == 0)
-          ok = bar_wait(&s.k_full[st ^ 1], ((it + 1) >> 1) & 1, &s.gone, a.err);
-        if (!ok) break;
-        scores(t, n + 2);
-      }
-    }
-    if (ok && b == 1) {
-      commit(&s.v_empty[st]);
-      if (n + 2 < halves) commit(&s.k_empty[st ^ 1]);
+      values(2 * it + b);
+      if (b == 1) commit(&s.v_empty[st]);
+      if (!more) continue;
+      if (b == 0) ok = bar_wait(&s.k_full[st ^ 1], ((it + 1) >> 1) & 1, &s.gone, a.err);
+      if (!ok) break;
+      scores(2 * it + 2 + b);
+      if (b == 1) commit(&s.k_empty[st ^ 1]);
     }
   }
   // also after a wait ran out: what was issued completes before TMEM is freed
@@ -493,6 +498,7 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   const uint32_t s_at = s.tmem + lanes + t * kTile, o_at = s.tmem + lanes + 256 + t * D;
   float M = kNoKey, l = 0.0f;
   bool ok = true;
+#pragma unroll 1
   for (int n = 0; n < 2 * sp.tiles; ++n) {
     const int it = n >> 1, b = n & 1, key0 = sp.first + n * kHalf;
     if (b == 0) ok = bar_wait(&s.place_full[it % kRing], (it / kRing) & 1, &s.gone, a.err);
@@ -648,6 +654,7 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
 template <int D, typename T>
 __device__ __forceinline__ void nothing(const AttendArgs& a, const Request& rq, int h, int m0,
                                         int split, int all) {
+#pragma unroll 1
   for (int i = threadIdx.x; i < min(2 * kTile, all - m0); i += kCta) {
     const int m = m0 + i;
     const int64_t tok = rq.q0 + m / a.group;
@@ -657,6 +664,7 @@ __device__ __forceinline__ void nothing(const AttendArgs& a, const Request& rq, 
       continue;
     }
     T* dst = static_cast<T*>(a.out) + tok * a.o_tok + hq * a.o_head;
+#pragma unroll 1
     for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     if (a.lse != nullptr) a.lse[tok * a.hq + hq] = -INFINITY;
   }
@@ -704,9 +712,9 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
     bar_init(&s.q_full, 8);  // one arrival a warp
     for (int i = 0; i < 2; ++i) {
       bar_init(&s.k_full[i], 4);
-      bar_init(&s.k_empty[i], 1);
+      bar_init(&s.k_empty[i], two ? 2 : 1);  // an arrival a row tile
       bar_init(&s.v_full[i], 4);
-      bar_init(&s.v_empty[i], 1);
+      bar_init(&s.v_empty[i], two ? 2 : 1);
       for (int b = 0; b < 2; ++b) {
         bar_init(&s.s_full[i][b], 1);
         bar_init(&s.p_full[i][b], 4);
@@ -717,7 +725,7 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
       bar_init(&s.place_full[i], 2);
       bar_init(&s.place_empty[i], two ? 12 : 8);  // softmax warps of live tiles, loaders
     }
-    bar_init(&s.done, 1);
+    bar_init(&s.done, two ? 2 : 1);
     s.gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -740,15 +748,16 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
     loader<D>(a, s, h, sp.tiles);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 12) {
-      if (elect_one()) {
-        issuer<D>(a, s, sp.tiles, two);
+    if (warp < 14) {
+      if ((warp == 12 || two) && elect_one()) {
+        issuer<D>(a, s, sp.tiles, warp - 12);
         // after a wait that ran out nobody else waits for the products
+#pragma unroll 1
         for (uint32_t i = 0; i < kRounds && !bar_try(&s.done, 0); ++i) {
         }
       }
       __syncwarp();
-    } else if (warp < 15) {
+    } else {
       finder<D, PAGE16>(a, s, r, h, sp);
     }
   }
