@@ -449,44 +449,59 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   see.x = max(see.x, sp.lo);
   see.y = min(see.y, sp.hi);
 
-  // the warp's query rows, a row on D / 8 lanes: f16 after a power of two
+  // The warp's query rows, a row on D / 8 lanes: copied as they are, then made f16 after a power of two
+  // in place.  The loops stay rolled: this code runs once a CTA, and fetching it costs more than it.
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a warp-wide load
-  constexpr int kAhead = 8;                           // loads in flight
   const int64_t q_row = tok * a.q_tok + hq * a.q_head;  // of this lane's row; others' by shuffle
+  constexpr int kBatch = 4;
+#pragma unroll 4
+  for (int i = 0; i < 32; i += kRows) {
+    const int from = i + lane / kLanes;
+    const T* src = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, q_row, from) + lane % kLanes * 8;
+    // rows past the last are zeros: a copy of no bytes fills with them
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(
+                     s.q[t] + tile_at<D>((warp & 3) * 32 + from, lane % kLanes))),
+                 "l"(src), "r"(from < mine ? 16 : 0)
+                 : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-  for (int i0 = 0; i0 < kLanes; i0 += kAhead) {
-    uint4 w[kAhead];
+  for (int i = 0; i < 32; i += kBatch * kRows) {
+    uint4 w[kBatch];
+    float top[kBatch];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int from = (i0 + i) * kRows + lane / kLanes;
-      const int64_t at = __shfl_sync(0xffffffffu, q_row, from);
-      w[i] = make_uint4(0, 0, 0, 0);
-      if (from < mine)
-        w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + lane % kLanes);
+    for (int j = 0; j < kBatch; ++j)
+      w[j] = *reinterpret_cast<const uint4*>(
+          s.q[t] + tile_at<D>((warp & 3) * 32 + i + j * kRows + lane / kLanes, lane % kLanes));
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      // the largest magnitude: both 16-bit types order as their bits do without the sign
+      uint32_t m = __vmaxu2(__vmaxu2(w[j].x & 0x7fff7fff, w[j].y & 0x7fff7fff),
+                            __vmaxu2(w[j].z & 0x7fff7fff, w[j].w & 0x7fff7fff));
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d /= 2) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+      float f[2];
+      Elem<T>::unpack(__vmaxu2(m, m >> 16), f);
+      top[j] = f[0];
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = (warp & 3) * 32 + (i0 + i) * kRows + lane / kLanes;
-      float f[8];
-      Elem<T>::unpack(w[i].x, f);
-      Elem<T>::unpack(w[i].y, f + 2);
-      Elem<T>::unpack(w[i].z, f + 4);
-      Elem<T>::unpack(w[i].w, f + 6);
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-#pragma unroll
-      for (int d = kLanes / 2; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+    for (int j = 0; j < kBatch; ++j) {
+      const int r = (warp & 3) * 32 + i + j * kRows + lane / kLanes;
+      int e2 = (int)(__float_as_uint(top[j]) >> 23) - 127;
       if (e2 < -126 || e2 > 126) e2 = 0;
       const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+      const uint32_t in[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+      uint32_t to[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= down;
-      *reinterpret_cast<uint4*>(s.q[t] + tile_at<D>(at, lane % kLanes)) =
-          make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]),
-                     pack_f16x2(f[6], f[7]));
+      for (int e = 0; e < 4; ++e) {
+        float f[2];
+        Elem<T>::unpack(in[e], f);
+        to[e] = pack_f16x2(f[0] * down, f[1] * down);
+      }
+      *reinterpret_cast<uint4*>(s.q[t] + tile_at<D>(r, lane % kLanes)) =
+          make_uint4(to[0], to[1], to[2], to[3]);
       if (lane % kLanes == 0)
-        s.up[t][at] = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
+        s.up[t][r] = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
     }
   }
   fence_smem();
@@ -614,7 +629,7 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   // Rows go through shared memory (K's and V's, done with), so that whole rows are written: 32 rows of
   // D words a warp, 16-byte chunks swizzled by row.
   float4* stage = reinterpret_cast<float4*>((t ? s.v : s.k)[0]) + (warp & 3) * (32 * D / 4);
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < D; c += 32) {
     uint32_t o[32];
     tmem_load32(o_at + c, o);
@@ -633,20 +648,32 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   const float mul = !any ? 0.0f : parts ? 1.0f : by;
   T* out = static_cast<T*>(a.out) + lane % kLanesOut * 4;
   float* part_o = a.rpart_o + lane % kLanesOut * 4;
-#pragma unroll 4
-  for (int i = 0; i < kLanesOut; ++i) {
-    const int from = i * (32 / kLanesOut) + lane / kLanesOut;
-    float4 y = stage[from * kLanesOut + (lane % kLanesOut ^ (from & 7))];
-    const int64_t to = __shfl_sync(0xffffffffu, o_row, from);
-    const float scale = __shfl_sync(0xffffffffu, mul, from);
-    if (from >= mine) continue;
-    // a row without keys is zeros, whatever the values beside it were
-    y = scale == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                      : make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
-    if (parts)
-      *reinterpret_cast<float4*>(part_o + to) = y;
-    else
-      *reinterpret_cast<uint2*>(out + to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+#pragma unroll 1
+  for (int i = 0; i < kLanesOut; i += kBatch) {
+    float4 y[kBatch];
+    int64_t to[kBatch];
+    float scale[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int from = (i + j) * (32 / kLanesOut) + lane / kLanesOut;
+      y[j] = stage[from * kLanesOut + (lane % kLanesOut ^ (from & 7))];
+      to[j] = __shfl_sync(0xffffffffu, o_row, from);
+      scale[j] = __shfl_sync(0xffffffffu, mul, from);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int from = (i + j) * (32 / kLanesOut) + lane / kLanesOut;
+      // a row without keys is zeros, whatever the values beside it were
+      const float4 z = scale[j] == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                        : make_float4(y[j].x * scale[j], y[j].y * scale[j],
+                                                      y[j].z * scale[j], y[j].w * scale[j]);
+      if (from < mine) {
+        if (parts)
+          *reinterpret_cast<float4*>(part_o + to[j]) = z;
+        else
+          *reinterpret_cast<uint2*>(out + to[j]) = make_uint2(pack2<T>(z.x, z.y), pack2<T>(z.z, z.w));
+      }
+    }
   }
 }
 
