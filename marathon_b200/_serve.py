@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -12,47 +11,54 @@ from ._lib import ShiftError
 from .paged import PagedLayout, describe
 from .shift_kernels import _ERR, _err_word, _raise_bits, take_errors
 
-_NO_GUARD = contextlib.nullcontext()
+
+def cuda_on(names: str, *tensors: torch.Tensor | None) -> int:
+    """Every tensor given (named in order by ``names``, None left out) is on one CUDA device,
+    whose index is returned."""
+    at = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i < 0 or i != at >= 0:
+                name = names.split()[next(j for j, x in enumerate(tensors) if x is t)]
+                if i < 0:
+                    raise ShiftError(f"{name} is on {t.device}: the kernels are CUDA-only and have no "
+                                     "CPU path")
+                raise ShiftError(f"{name} is on {t.device}, other arguments are on cuda:{at}")
+            at = i
+    return at
 
 
-def cuda_on(device: torch.device | None, **tensors: torch.Tensor | None) -> torch.device:
-    """Every tensor given is on one CUDA device (``device`` if not None), which is returned."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ShiftError(f"{name} is on {t.device}: the kernels are CUDA-only and have no "
-                             "CPU path")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ShiftError(f"{name} is on {t.device}, other arguments are on {device}")
-    return device
-
-
-def refuse_grad(what: str, hint: str, *tensors: torch.Tensor | None) -> None:
+def refuse_grad(what: str, hint: str) -> None:
     """These operators record no gradient; a caller who would lose one is told."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled():
         raise ShiftError(f"{what} records no gradient: {hint}")
 
 
-def int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
-        raise ShiftError(f"{name} must be a contiguous int32 vector, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    if numel is not None and t.numel() != numel:
-        raise ShiftError(f"{name} has {t.numel()} entries, {numel} are wanted")
+def int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> int:
+    """Its length, which is ``numel`` if that is given."""
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != 1 or (shape[0] > 1 and t.stride(0) != 1):
+        raise ShiftError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(shape)}")
+    n = shape[0]
+    if numel is not None and n != numel:
+        raise ShiftError(f"{name} has {n} entries, {numel} are wanted")
+    return n
 
 
-def block_table_rows(t: torch.Tensor) -> tuple[int, int]:
-    """(row stride, width) of an int32 ``[requests, width]`` block table."""
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+def block_table_rows(t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, row stride, width) of an int32 ``[requests, width]`` block table."""
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != 2 or (shape[1] > 1 and t.stride(1) != 1):
         raise ShiftError("block_tables must be int32 [requests, width] with contiguous rows, got "
-                         f"{t.dtype} {tuple(t.shape)}")
-    width = t.shape[1]
-    if t.shape[0] > 1 and t.stride(0) < width:
+                         f"{t.dtype} {tuple(shape)}")
+    rows, width = shape
+    if rows <= 1:
+        return rows, width, width
+    stride = t.stride(0)
+    if stride < width:
         raise ShiftError("block_tables' rows overlap")
-    return (t.stride(0) if t.shape[0] > 1 else width), width
+    return rows, stride, width
 
 
 def span(t: torch.Tensor) -> tuple[int, int]:
@@ -71,13 +77,14 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def heads_rows(t: torch.Tensor, name: str, written: bool = False) -> tuple[int, int]:
     """(token, head) strides of a ``[tokens, heads, head_size]`` tensor with contiguous heads."""
-    if t.dim() != 3:
+    stride = t.stride()
+    if len(stride) != 3:
         raise ShiftError(f"{name} must be [tokens, heads, head_size], got {tuple(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if stride[2] != 1 and t.shape[2] > 1:
         raise ShiftError(f"{name}'s head dimension must be contiguous")
-    if written and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride(), strict=True)):
+    if written and 0 in stride and any(n > 1 and s == 0 for n, s in zip(t.shape, stride, strict=True)):
         raise ShiftError(f"{name} is written and must not repeat its elements")
-    return t.stride(0), t.stride(1)
+    return stride[0], stride[1]
 
 
 _geometries: dict = {}
@@ -105,45 +112,42 @@ def geometry(kv: torch.Tensor, block_size: int, layout: str | None) -> tuple[Pag
 
 
 def scale_strides(scale: torch.Tensor, geo: PagedLayout, name: str) -> tuple[int, int]:
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (geo.num_blocks, geo.heads):
+    if scale.dtype is not torch.float32 or scale.shape != (geo.num_blocks, geo.heads):
         raise ShiftError(f"{name} must be fp32 [{geo.num_blocks}, {geo.heads}] (blocks, heads), "
                          f"got {scale.dtype} {tuple(scale.shape)}")
-    return scale.stride(0), scale.stride(1)
+    return scale.stride()
 
 
-def status_word(device: torch.device) -> torch.Tensor:
-    """The device's status word (``take_errors`` reads and clears it)."""
-    if device.index not in _ERR:
-        if torch.cuda.is_current_stream_capturing():
-            raise ShiftError("call the operator once on this device before capturing it: its "
-                             "status word must not live in a graph's memory")
+_status: dict[int, int] = {}  # device index -> address of its status word
+
+
+def _status_word(index: int) -> int:
+    """Address of the device's status word (``take_errors`` reads and clears it)."""
+    if index not in _ERR and torch.cuda.is_current_stream_capturing():
+        raise ShiftError("call the operator once on this device before capturing it: its "
+                         "status word must not live in a graph's memory")
+    with torch.cuda.device(index):
+        at = _status[index] = _err_word(torch.device("cuda", index)).data_ptr()
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().synchronize()  # other streams may use it from now on
+    return at
+
+
+def launch(fn, what: str, device: int, args: tuple, check: bool) -> None:
+    """Call the entry point with the device's status word and current stream behind ``args``,
+    that device being current."""
+    err = _status.get(device) or _status_word(device)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch.cuda.current_device() == device:
+        status = fn(*args, err, stream)
+    else:
         with torch.cuda.device(device):
-            _err_word(device)
-            torch.cuda.current_stream().synchronize()
-    return _ERR[device.index]
+            status = fn(*args, err, stream)
+    if status or check:
+        finish(status, what, device, check)
 
 
-class Launch:
-    """The device's status word and current stream, with that device current inside ``with``."""
-
-    __slots__ = ("device", "err", "guard", "stream")
-
-    def __init__(self, device: torch.device) -> None:
-        self.device = device
-        self.err = status_word(device).data_ptr()
-        self.guard = (_NO_GUARD if torch.cuda.current_device() == device.index
-                      else torch.cuda.device(device))
-
-    def __enter__(self) -> Launch:
-        self.guard.__enter__()
-        self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        return self
-
-    def __exit__(self, *exc) -> None:
-        self.guard.__exit__(*exc)
-
-
-def finish(status: int, what: str, device: torch.device, check: bool) -> None:
+def finish(status: int, what: str, device: int, check: bool) -> None:
     _lib.check(status, what)
     if check:
-        _raise_bits(take_errors(device), what)
+        _raise_bits(take_errors(torch.device("cuda", device)), what)

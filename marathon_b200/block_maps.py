@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._serve import Launch, block_table_rows, cuda_on, finish, int32_vector, overlap
+from ._serve import block_table_rows, cuda_on, int32_vector, launch
 
 __all__ = ["BlockMaps", "block_maps"]
 
@@ -58,30 +58,30 @@ def block_maps(
     narrow, an old entry below 0, negative lengths (read as 0), more tokens than ``tokens``
     (the surplus is dropped, from ``seq_lens`` too).
     """
-    dev = cuda_on(None, cached_lens=cached_lens, new_lens=new_lens, block_tables=block_tables,
-                  free_blocks=free_blocks, free_head=free_head)
-    int32_vector(cached_lens, "cached_lens")
-    reqs = cached_lens.numel()
+    dev = cuda_on("cached_lens new_lens block_tables free_blocks free_head", cached_lens, new_lens,
+                  block_tables, free_blocks, free_head)
+    reqs = int32_vector(cached_lens, "cached_lens")
     int32_vector(new_lens, "new_lens", reqs)
-    int32_vector(free_blocks, "free_blocks")
+    n_free = int32_vector(free_blocks, "free_blocks")
     int32_vector(free_head, "free_head", 1)
-    stride, width = block_table_rows(block_tables)
-    if block_tables.shape[0] != reqs:
-        raise _lib.ShiftError(f"{block_tables.shape[0]} block tables for {reqs} requests")
+    n_tables, stride, width = block_table_rows(block_tables)
+    if n_tables != reqs:
+        raise _lib.ShiftError(f"{n_tables} block tables for {reqs} requests")
     if block_size <= 0 or not 0 <= tokens < 2**31:
         raise _lib.ShiftError(f"block_size {block_size} and tokens {tokens} must be positive int32s")
-    for name, t in (("cached_lens", cached_lens), ("new_lens", new_lens),
-                    ("free_blocks", free_blocks), ("free_head", free_head)):
-        if overlap(t, block_tables):
-            raise _lib.ShiftError(f"{name} shares memory with block_tables, which are written")
-    lib = _lib.load()
-    with Launch(dev) as on:
-        ints = [torch.empty(n, dtype=torch.int32, device=dev) for n in (reqs + 1, reqs, 1)]
-        rows = [torch.empty(tokens, dtype=torch.int64, device=dev) for _ in range(2)]
-        status = lib.mshift_block_maps(
-            cached_lens.data_ptr(), new_lens.data_ptr(), reqs, block_tables.data_ptr(), stride,
-            width, free_blocks.data_ptr(), free_blocks.numel(), free_head.data_ptr(), block_size,
-            tokens, ints[0].data_ptr(), ints[1].data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(),
-            ints[2].data_ptr(), on.err, on.stream)
-    finish(status, "block_maps", dev, check)
-    return BlockMaps(ints[0], ints[1], rows[0], rows[1], ints[2])
+    read = (cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), free_head.data_ptr())
+    table = block_tables.data_ptr()
+    end = table + 4 * ((reqs - 1) * stride + width)
+    for at, n in zip(read, (reqs, reqs, n_free, 1), strict=True):
+        if at < end and table < at + 4 * n:
+            raise _lib.ShiftError("an argument shares memory with block_tables, which are written")
+    query_start = cached_lens.new_empty(reqs + 1)
+    seq_lens = cached_lens.new_empty(reqs)
+    head = cached_lens.new_empty(1)
+    slots = cached_lens.new_empty(tokens, dtype=torch.int64)
+    positions = cached_lens.new_empty(tokens, dtype=torch.int64)
+    launch(_lib.load().mshift_block_maps, "block_maps", dev, (
+        read[0], read[1], reqs, table, stride, width, read[2], n_free, read[3], block_size, tokens,
+        query_start.data_ptr(), seq_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        head.data_ptr()), check)
+    return BlockMaps(query_start, seq_lens, slots, positions, head)

@@ -22,10 +22,10 @@ import torch
 
 from . import _lib
 from ._serve import (
-    Launch, block_table_rows, cuda_on, finish, geometry, heads_rows, int32_vector, overlap,
-    refuse_grad, scale_strides,
+    block_table_rows, cuda_on, geometry, heads_rows, int32_vector, launch, overlap, refuse_grad,
+    scale_strides,
 )
-from .paged import base_pointers, dtype_code
+from .paged import dtype_code
 
 __all__ = ["append_block_scaled", "attend_block_scaled"]
 
@@ -37,15 +37,15 @@ def _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
     geo, paged = geometry(kv, block_size, layout)
     if geo.head_size not in HEAD_SIZES:
         raise _lib.ShiftError(f"head_size {geo.head_size} is not one of {HEAD_SIZES}")
-    k_base, v_base = base_pointers(kv, geo)
+    k_base = kv.data_ptr()
     if k_base % 16:
         raise _lib.ShiftError("the cache must start on a 16-byte boundary")
-    ks, vs = scale_strides(k_scale, geo, "k_scale"), scale_strides(v_scale, geo, "v_scale")
-    stride, width = block_table_rows(block_tables)
-    reqs = block_tables.shape[0]
+    reqs, stride, width = block_table_rows(block_tables)
     int32_vector(query_start, "query_start", reqs + 1)
     int32_vector(seq_lens, "seq_lens", reqs)
-    cache = (paged, k_base, v_base, k_scale.data_ptr(), *ks, v_scale.data_ptr(), *vs)
+    cache = (paged, k_base, k_base + geo.v_offset, k_scale.data_ptr(),
+             *scale_strides(k_scale, geo, "k_scale"), v_scale.data_ptr(),
+             *scale_strides(v_scale, geo, "v_scale"))
     step = (block_tables.data_ptr(), stride, width, query_start.data_ptr(), seq_lens.data_ptr(), reqs)
     return geo, cache, step
 
@@ -77,33 +77,36 @@ def append_block_scaled(
     (copy a shared block before appending to it).  Flagged and skipped: a block outside
     the cache, positions past the block table, rows before position 0.
     """
-    dev = cuda_on(None, kv=kv, k=k, v=v, k_scale=k_scale, v_scale=v_scale,
-                  block_tables=block_tables, query_start=query_start, seq_lens=seq_lens)
-    refuse_grad("append_block_scaled", "detach k and v", k, v)
+    dev = cuda_on("k v kv k_scale v_scale block_tables query_start seq_lens", k, v, kv, k_scale, v_scale,
+                  block_tables, query_start, seq_lens)
+    if k.requires_grad or v.requires_grad:
+        refuse_grad("append_block_scaled", "detach k and v")
     geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
                              layout)
     code = dtype_code(k.dtype)
     if code == _lib.E4M3 or v.dtype != k.dtype:
         raise _lib.ShiftError(f"k and v must both be bf16, fp16 or fp32, got {k.dtype} and {v.dtype}")
-    rows = []
-    for name, t in (("k", k), ("v", v)):
-        rows += [t.data_ptr(), *heads_rows(t, name)]
-        if tuple(t.shape) != (k.shape[0], geo.heads, geo.head_size):
+    n = k.shape[0]
+    want = (n, geo.heads, geo.head_size)
+    k_rows, v_rows = (k.data_ptr(), *heads_rows(k, "k")), (v.data_ptr(), *heads_rows(v, "v"))
+    vec = 4 if code == _lib.F32 else 8
+    for name, t, (at, tok, head) in (("k", k, k_rows), ("v", v, v_rows)):
+        if t.shape != want:
             raise _lib.ShiftError(f"{name} must be [tokens, {geo.heads}, {geo.head_size}], got "
                                   f"{tuple(t.shape)}")
-        vec = 16 // t.element_size()
-        if t.data_ptr() % 16 or t.stride(0) % vec or t.stride(1) % vec:
+        if at % 16 or tok % vec or head % vec:
             raise _lib.ShiftError(f"{name}'s rows must start on 16-byte boundaries")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride(), strict=True)):
-            raise _lib.ShiftError(f"{name} is written and must not repeat its elements")
-    if k_scale.data_ptr() == v_scale.data_ptr() and k_scale.numel():
+    if 0 in cache[4:6] or 0 in cache[7:9]:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if any(m > 1 and s == 0 for m, s in zip(t.shape, t.stride(), strict=True)):
+                raise _lib.ShiftError(f"{name} is written and must not repeat its elements")
+    if cache[3] == cache[6] and k_scale.numel():
         raise _lib.ShiftError("k_scale and v_scale must be two tensors")
-    lib = _lib.load()
-    with Launch(dev) as on:
-        status = lib.mshift_append_block_scaled(code, *rows, k.shape[0], *cache, *step, on.err,
-                                                on.stream)
-    finish(status, "append_block_scaled", dev, check)
+    launch(_lib.load().mshift_append_block_scaled, "append_block_scaled", dev,
+           (code, *k_rows, *v_rows, n, *cache, *step), check)
+
+
+_workspaces: dict[tuple, int] = {}  # shapes of a call -> bytes of workspace it needs
 
 
 def attend_block_scaled(
@@ -146,54 +149,64 @@ def attend_block_scaled(
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
     the bounds (cut off there), positions past the block table (unseen).
     """
-    dev = cuda_on(None, q=q, kv=kv, k_scale=k_scale, v_scale=v_scale, block_tables=block_tables,
-                  query_start=query_start, seq_lens=seq_lens, out=out)
-    refuse_grad("attend_block_scaled", "a cache of codes is not trained through", q, out)
+    dev = cuda_on("q kv k_scale v_scale block_tables query_start seq_lens out", q, kv, k_scale, v_scale,
+                  block_tables, query_start, seq_lens, out)
+    if q.requires_grad or (out is not None and out.requires_grad):
+        refuse_grad("attend_block_scaled", "a cache of codes is not trained through")
     geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
                              layout)
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dtype is torch.bfloat16:
+        code = _lib.BF16
+    elif q.dtype is torch.float16:
+        code = _lib.F16
+    else:
         raise _lib.ShiftError(f"q must be bf16 or fp16, got {q.dtype}")
     q_tok, q_head = heads_rows(q, "q")
     rows, hq, head_size = q.shape
     if head_size != geo.head_size or hq == 0 or hq % geo.heads:
         raise _lib.ShiftError(f"q {tuple(q.shape)} does not fit {geo.heads} heads of {geo.head_size}")
-    if q.data_ptr() % 16 or q_tok % 8 or q_head % 8:
+    q_at = q.data_ptr()
+    if q_at % 16 or q_tok % 8 or q_head % 8:
         raise _lib.ShiftError("q's rows must start on 16-byte boundaries")
     if not 0 <= max_query_len < 2**31 or not 0 <= max_seq_len < 2**31 or not 0 <= window < 2**31:
         raise _lib.ShiftError("max_query_len, max_seq_len and window must be non-negative int32s")
     scale = head_size ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise _lib.ShiftError(f"scale must be finite, got {scale}")
+    reqs = step[-1]
+    lse = None
     zero_tail = out is None
-    if out is not None:
-        heads_rows(out, "out", written=True)
-        if out.shape != q.shape or out.dtype != q.dtype:
+    if zero_tail:
+        # the kernels write every row, unless there is no request and so no kernel
+        out = q.new_empty((rows, hq, head_size)) if reqs else q.new_zeros((rows, hq, head_size))
+        o_tok, o_head = hq * head_size, head_size
+        if return_lse:
+            lse = q.new_empty((rows, hq), dtype=torch.float32)
+            if not reqs:
+                lse.fill_(-math.inf)
+    else:
+        o_tok, o_head = heads_rows(out, "out", written=True)
+        if out.shape != q.shape or out.dtype is not q.dtype:
             raise _lib.ShiftError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} "
                                   f"{tuple(out.shape)}")
-        if out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8:
+        if out.data_ptr() % 16 or o_tok % 8 or o_head % 8:
             raise _lib.ShiftError("out's rows must start on 16-byte boundaries")
         for name, t in (("q", q), ("kv", kv), ("k_scale", k_scale), ("v_scale", v_scale)):
             if overlap(out, t):
                 raise _lib.ShiftError(f"out shares memory with {name}")
+        if return_lse:  # rows behind the last request have -inf where out keeps what it held
+            lse = q.new_full((rows, hq), -math.inf, dtype=torch.float32)
     lib = _lib.load()
-    code = dtype_code(q.dtype)
-    reqs = step[-1]
-    with Launch(dev) as on:
-        if out is None:
-            make = torch.zeros if reqs == 0 else torch.empty
-            out = make(q.shape, dtype=q.dtype, device=dev)
-        lse = None
-        if return_lse:
-            # rows behind the last request keep -inf where out keeps what it held
-            lse = (torch.empty if zero_tail and reqs else torch.full)(
-                (rows, hq), *(() if zero_tail and reqs else (-math.inf,)), dtype=torch.float32, device=dev)
-        need = lib.mshift_attend_workspace(rows, hq, geo.heads, head_size, reqs, max_query_len,
-                                           max_seq_len)
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        status = lib.mshift_attend_block_scaled(
-            code, q.data_ptr(), q_tok, q_head, rows, hq, *cache, *step, max_query_len, max_seq_len,
-            scale, int(causal), window, out.data_ptr(), out.stride(0), out.stride(1),
-            None if lse is None else lse.data_ptr(), int(zero_tail),
-            None if work is None else work.data_ptr(), max(need, 0), on.err, on.stream)
-    finish(status, "attend_block_scaled", dev, check)
+    key = (rows, hq, geo.heads, head_size, reqs, max_query_len, max_seq_len)
+    need = _workspaces.get(key)
+    if need is None:
+        if len(_workspaces) > 4096:
+            _workspaces.clear()
+        need = _workspaces[key] = max(lib.mshift_attend_workspace(*key), 0)
+    # from the caching allocator, on this stream: calls and graphs do not share it
+    work = q.new_empty(need, dtype=torch.uint8) if need else None
+    launch(lib.mshift_attend_block_scaled, "attend_block_scaled", dev, (
+        code, q_at, q_tok, q_head, rows, hq, *cache, *step, max_query_len, max_seq_len, scale,
+        int(causal), window, out.data_ptr(), o_tok, o_head, None if lse is None else lse.data_ptr(),
+        int(zero_tail), None if work is None else work.data_ptr(), need), check)
     return (out, lse) if return_lse else out

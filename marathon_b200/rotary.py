@@ -16,7 +16,7 @@ from collections.abc import Sequence
 import torch
 
 from . import _lib
-from ._serve import Launch, cuda_on, finish, heads_rows, int32_vector, overlap, refuse_grad
+from ._serve import cuda_on, heads_rows, int32_vector, launch, overlap, refuse_grad
 from .paged import dtype_code
 
 __all__ = ["axis_map", "rotary_axes"]
@@ -66,30 +66,38 @@ def rotary_axes(
     one = q if q is not None else k
     if one is None:
         raise _lib.ShiftError("rotary_axes needs q or k")
-    dev = cuda_on(None, q=q, k=k, positions=positions, inv_freq=inv_freq, axes=axes)
-    refuse_grad("rotary_axes", "its gradient is rotary_axes(..., inverse=True) of the result's", q, k)
+    dev = cuda_on("q k positions inv_freq axes", q, k, positions, inv_freq, axes)
+    if one.requires_grad or (k is not None and k.requires_grad):
+        refuse_grad("rotary_axes", "its gradient is rotary_axes(..., inverse=True) of the result's, and "
+                    "torch.ops.marathon.rotary_axes records it")
     code = dtype_code(one.dtype)
     if code == _lib.E4M3:
         raise _lib.ShiftError("rotary_axes takes bf16, fp16 or fp32")
-    if one.dim() != 3:
-        raise _lib.ShiftError(f"q and k must be [tokens, heads, head_size], got {tuple(one.shape)}")
-    n, _, head_size = one.shape
-    if q is not None and k is not None and (k.dtype != q.dtype or k.dim() != 3
-                                            or k.shape[0] != n or k.shape[2] != head_size):
-        raise _lib.ShiftError(f"q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} differ in "
-                              "type, tokens or head size")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+    shape = one.shape
+    if len(shape) != 3:
+        raise _lib.ShiftError(f"q and k must be [tokens, heads, head_size], got {tuple(shape)}")
+    n, _, head_size = shape
+    hq = 0 if q is None else shape[1]
+    hk = 0
+    if k is not None:
+        kshape = k.shape
+        if k.dtype is not one.dtype or len(kshape) != 3 or kshape[0] != n or kshape[2] != head_size:
+            raise _lib.ShiftError(f"q {one.dtype} {tuple(shape)} and k {k.dtype} {tuple(kshape)} differ "
+                                  "in type, tokens or head size")
+        hk = kshape[1]
+    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1:
         raise _lib.ShiftError("inv_freq must be an fp32 vector")
     half = inv_freq.numel()
     if 2 * half > head_size:
         raise _lib.ShiftError(f"rotary {2 * half} > head_size {head_size}")
     if half > 256 or head_size > 1024:
         raise _lib.ShiftError("rotary_axes takes head sizes up to 1024 and rotary up to 512")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
-            or positions.shape[-1] != n:
+    pshape = positions.shape
+    if positions.dtype not in (torch.int32, torch.int64) or len(pshape) not in (1, 2) \
+            or pshape[-1] != n:
         raise _lib.ShiftError(f"positions must be int32 or int64 [{n}] or [axes, {n}], got "
-                              f"{positions.dtype} {tuple(positions.shape)}")
-    n_axes = positions.shape[0] if positions.dim() == 2 else 1
+                              f"{positions.dtype} {tuple(pshape)}")
+    n_axes = pshape[0] if len(pshape) == 2 else 1
     if n_axes == 0:
         raise _lib.ShiftError("positions have no axis")
     if axes is not None:
@@ -100,33 +108,29 @@ def rotary_axes(
         positions = positions.contiguous()
     if half > 1 and inv_freq.stride(0) != 1:
         inv_freq = inv_freq.contiguous()
-    ins, outs = [], []
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            ins += [None, 0, 0]
-            continue
-        ins += [t.data_ptr(), *heads_rows(t, name, inplace)]
-    if inplace and q is not None and k is not None and overlap(q, k) and _interleaved_clash(q, k):
-        raise _lib.ShiftError("q and k share elements and cannot both be rotated in place")
+    q_in = (None, 0, 0) if q is None else (q.data_ptr(), *heads_rows(q, "q", inplace))
+    k_in = (None, 0, 0) if k is None else (k.data_ptr(), *heads_rows(k, "k", inplace))
     if inplace:
+        if q is not None and k is not None and overlap(q, k) and _interleaved_clash(q, k):
+            raise _lib.ShiftError("q and k share elements and cannot both be rotated in place")
         for t in (positions, inv_freq, axes):
             if t is not None and any(x is not None and overlap(t, x) for x in (q, k)):
                 raise _lib.ShiftError("an argument shares memory with a tensor rotated in place")
-    lib = _lib.load()
-    with Launch(dev) as on:
-        got = []
-        for t in (q, k):
-            o = t if t is None or inplace else torch.empty(t.shape, dtype=t.dtype, device=dev)
-            got.append(o)
-            outs += [None, 0, 0] if o is None else [o.data_ptr(), o.stride(0), o.stride(1)]
-        status = lib.mshift_rotary_axes(
-            code, *ins[:3], *outs[:3], 0 if q is None else q.shape[1], *ins[3:], *outs[3:],
-            0 if k is None else k.shape[1], n, head_size, 2 * half, positions.data_ptr(),
-            positions.stride(0) if n_axes > 1 else n, int(positions.dtype == torch.int64), n_axes,
-            inv_freq.data_ptr(), None if axes is None else axes.data_ptr(), int(inverse), on.err,
-            on.stream)
-    finish(status, "rotary_axes", dev, check)
-    return got[0], got[1]
+        q_out, k_out, q_to, k_to = q, k, q_in, k_in
+    else:
+        q_out = q_to = k_out = k_to = None
+        if q is not None:
+            q_out = q.new_empty(shape)
+            q_to = (q_out.data_ptr(), hq * head_size, head_size)
+        if k is not None:
+            k_out = k.new_empty(k.shape)
+            k_to = (k_out.data_ptr(), hk * head_size, head_size)
+    launch(_lib.load().mshift_rotary_axes, "rotary_axes", dev, (
+        code, *q_in, *(q_to or q_in), hq, *k_in, *(k_to or k_in), hk, n, head_size, 2 * half,
+        positions.data_ptr(), positions.stride(0) if n_axes > 1 else n,
+        int(positions.dtype is torch.int64), n_axes, inv_freq.data_ptr(),
+        None if axes is None else axes.data_ptr(), int(inverse)), check)
+    return q_out, k_out
 
 
 def _interleaved_clash(q: torch.Tensor, k: torch.Tensor) -> bool:
