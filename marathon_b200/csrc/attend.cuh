@@ -36,6 +36,7 @@ struct AttendArgs {
   int64_t blk, off, head;  // cache strides, bytes
   int64_t num_blocks;
   int bs;
+  uint32_t bs_mul, bs_shift;  // t / bs = (high word of t * mul, + t) >> shift for t below 2^31
   const float* ks;
   const float* vs;
   int64_t ks_blk, ks_head, vs_blk, vs_head;
@@ -66,6 +67,18 @@ struct AttendArgs {
   int max_q;     // the caller's bound on a request's tokens
   uint32_t* err;
 };
+
+// Division by the block size as a multiplication by its rounded-up reciprocal (Granlund and
+// Montgomery 1994): exact for every t below 2^31.
+inline void set_block_size(AttendArgs& a, int bs) {
+  a.bs = bs;
+  a.bs_shift = 0;
+  while ((1ll << a.bs_shift) < bs) ++a.bs_shift;
+  a.bs_mul = (uint32_t)((((1ull << a.bs_shift) - (uint64_t)bs) << 32) / (uint64_t)bs + 1);
+}
+__device__ __forceinline__ int block_column(const AttendArgs& a, int t) {
+  return (int)((__umulhi((uint32_t)t, a.bs_mul) + (uint32_t)t) >> a.bs_shift);
+}
 
 // One request's lengths, bounded by what the call's arrays hold.
 struct Request {

@@ -15,8 +15,10 @@
 //   values  O^T[16 dims x 8 rows] += V^T[16 dims x 16 tokens] P^T.  Lane (g, c) loads the
 //           codes of tokens 2c, 2c+1, 2c+8, 2c+9 at D/8 contiguous dims from g D/8; byte pairs of two
 //           tokens are the f16 pairs that the fragment wants.
-// P^T's fragment is S^T's transposed, which movmatrix does in registers.  The next step's codes are
-// loaded before this step's are used, so each warp keeps 16 tokens (4 KB at D = 128) in flight.
+// P^T's fragment is S^T's transposed, which movmatrix does in registers.  Codes and scales come
+// through a ring of stages in shared memory that each warp fills for itself with asynchronous
+// copies, three steps (12 KB at D = 128) ahead of the one it works on; chunks of 16 bytes are swizzled so that
+// the fragments' reads hit every bank once.
 #include "attend.cuh"
 
 namespace mshift {
@@ -43,34 +45,46 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// What a lane holds of one 16-token step.
+__device__ __forceinline__ void copy16(void* to, const void* from, bool take) {  // or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from), "r"(take ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from)
+               : "memory");
+}
+
+// One 16-token step of a warp.
 template <int D>
-struct Step {
-  static constexpr int kK = D / 64;                    // 16-byte loads of a K row
-  static constexpr int kV = D >= 128 ? D / 128 : 1;    // loads of a V row (8 bytes at D = 64)
-  uint4 k[2][kK];
-  uint4 v[4][kV];
-  float ks[2], vs[2];  // scales of tokens g and g + 8
+struct Stage {
+  uint8_t k[16 * D], v[16 * D];
+  float ks[16], vs[16];  // a block's at its first token's place, or each token's
+  static constexpr int kCopies = D / 32;  // 16-byte copies a lane, K or V
+  // place of 16-byte chunk c of token t
+  __device__ static int k_at(int t, int c) { return t * D + ((c ^ (D > 64 ? (t & 1) * 4 : 0)) << 4); }
+  __device__ static int v_at(int t, int c) {
+    return t * D + ((c ^ (D > 64 ? (t >> 1 & 3) * 2 : (t >> 1 & 1) * 2)) << 4);
+  }
 };
+template <int D>
+constexpr int kStages = D == 256 ? 2 : 3;
 
 template <int D, int NT, bool PAGE16, typename T>
 __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArgs a, int tiles) {
   constexpr int kRows = NT * 8;
   constexpr int kMt = D / 16;  // 16-dim tiles of O^T
+  constexpr int kS = kStages<D>;
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-  __shared__ float s_o[kWarps][kRows][D + 4];
+  float(*s_o)[kRows][D + 4] = reinterpret_cast<float(*)[kRows][D + 4]>(ring);  // after the last step
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -171,107 +185,105 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
   const float* vsh = a.vs + h * a.vs_head;
   const int first = lo < hi ? lo / 16 : 0, steps = lo < hi ? (hi + 15) / 16 - first : 0;
 
-  // Loads step st's codes and scales; tokens outside [lo, hi) or in a bad block
-  // load nothing and count as zero codes, which their mask leaves out.  Returns
-  // the tokens (16 bits) whose block is good.
-  auto fetch = [&](int st, Step<D>& x) -> unsigned {
-    const int t0 = (first + st) * 16;
-    unsigned good;
-    long long base = 0;  // PAGE16: the step's place in its block; else that of token lane & 15
-    float ks = 0.0f, vs = 0.0f;
-    {
-      const int t = PAGE16 ? t0 : t0 + (lane & 15);
-      const int col = t / a.bs;
-      bool ok = PAGE16 || (t >= lo && t < hi);
-      if (ok) {
-        const int b = table[col];
-        ok = b >= 0 && b < a.num_blocks;
-        if (ok) {
-          base = b * a.blk + (t - col * a.bs) * a.off;
-          ks = ksh[b * a.ks_blk];
-          vs = vsh[b * a.vs_blk];
-        } else {
-          flag(a.err, MSHIFT_EBIT_SLOT);
-        }
+  Stage<D>* stage = reinterpret_cast<Stage<D>*>(ring) + (threadIdx.x >> 5) * kS;
+  // Where step st's tokens lie: the step's block (PAGE16), or that of token lane & 15; -1 for
+  // a bad block or nothing to read.
+  auto block_of = [&](int st) -> int {
+    const int t = (first + st) * 16 + (PAGE16 ? 0 : lane & 15);
+    if (st >= steps || (!PAGE16 && (t < lo || t >= hi))) return -1;
+    const int b = table[block_column(a, t)];
+    if (b >= 0 && b < a.num_blocks) return b;
+    flag(a.err, MSHIFT_EBIT_SLOT);
+    return -1;
+  };
+  // Starts the copies of step st; tokens outside [lo, hi) or in a bad block are zeros, and a bad
+  // block's value scale is -1.
+  auto fetch = [&](int st, int b) {
+    if (st < steps) {
+      Stage<D>& x = stage[st / kWarps % kS];
+      const int t0 = (first + st) * 16, mine = t0 + (PAGE16 ? 0 : lane & 15);
+      const long long base = b * a.blk + (mine - block_column(a, mine) * a.bs) * a.off;
+      unsigned in = PAGE16 ? (b >= 0 ? 0xffffu : 0u) : __ballot_sync(0xffffffffu, b >= 0) & 0xffffu;
+      if (t0 < lo) in &= 0xffffu << (lo - t0);
+      if (t0 + 16 > hi) in &= 0xffffu >> (t0 + 16 - hi);
+#pragma unroll
+      for (int i = 0; i < Stage<D>::kCopies; ++i) {
+        const int q = lane + 32 * i, t = q / (D / 16), c = q % (D / 16);
+        const bool take = (in >> t) & 1;
+        const long long at =
+            (PAGE16 ? base + t * a.off : __shfl_sync(0xffffffffu, base, t)) + 16 * c;
+        copy16(x.k + Stage<D>::k_at(t, c), take ? kh + at : kh, take);
+        copy16(x.v + Stage<D>::v_at(t, c), take ? vh + at : vh, take);
       }
-      if (PAGE16)
-        good = ok ? 0xffffu : 0u;
-      else
-        good = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-    }
-    unsigned in = good;  // tokens to load
-    if (t0 < lo) in &= 0xffffu << (lo - t0);
-    if (t0 + 16 > hi) in &= 0xffffu >> (t0 + 16 - hi);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int t = g + 8 * e;
-      const long long at = PAGE16 ? base + t * a.off : __shfl_sync(0xffffffffu, base, t);
-      x.ks[e] = PAGE16 ? ks : __shfl_sync(0xffffffffu, ks, t);
-      x.vs[e] = PAGE16 ? vs : __shfl_sync(0xffffffffu, vs, t);
-#pragma unroll
-      for (int u = 0; u < Step<D>::kK; ++u)
-        x.k[e][u] = (in >> t) & 1 ? load16(kh + at + 64 * u + 16 * c) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = 2 * c + (e & 1) + 8 * (e >> 1);
-      const long long at = PAGE16 ? base + t * a.off : __shfl_sync(0xffffffffu, base, t);
-#pragma unroll
-      for (int u = 0; u < Step<D>::kV; ++u) {
-        x.v[e][u] = make_uint4(0, 0, 0, 0);
-        if ((in >> t) & 1) {
-          if constexpr (D == 64) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(vh + at + 8 * g));
-            x.v[e][u].x = w.x;
-            x.v[e][u].y = w.y;
-          } else {
-            x.v[e][u] = load16(vh + at + 128 * u + 16 * g);
-          }
-        }
+      if (PAGE16 ? lane < 2 : true) {
+        const bool is_v = PAGE16 ? lane == 1 : lane >= 16;
+        float* to = (is_v ? x.vs : x.ks) + (PAGE16 ? 0 : lane & 15);
+        if (b >= 0)
+          copy4(to, is_v ? vsh + b * a.vs_blk : ksh + b * a.ks_blk);
+        else
+          *to = is_v ? -1.0f : 0.0f;
       }
     }
-    return good;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  Step<D> cur, nxt;
-  unsigned good = 0, good_nxt = 0;
-  if (warp < steps) good = fetch(warp, cur);
+  int ahead = block_of(warp);
+#pragma unroll 1
+  for (int i = 0; i < kS - 1; ++i) {
+    fetch(warp + i * kWarps, ahead);
+    ahead = block_of(warp + (i + 1) * kWarps);
+  }
+#pragma unroll 1
   for (int st = warp; st < steps; st += kWarps) {
-    if (st + kWarps < steps) good_nxt = fetch(st + kWarps, nxt);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kS - 2) : "memory");
+    __syncwarp();
+    fetch(st + (kS - 1) * kWarps, ahead);
+    ahead = block_of(st + kS * kWarps);
+    const Stage<D>& cur = stage[st / kWarps % kS];
     const int t0 = (first + st) * 16;
 
     float s[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const uint32_t w0 = word(cur.k[0][d / 4], d % 4), w1 = word(cur.k[1][d / 4], d % 4);
-      const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)w0), e4m3x2_to_f16x2((uint16_t)w1),
-                             e4m3x2_to_f16x2((uint16_t)(w0 >> 16)),
-                             e4m3x2_to_f16x2((uint16_t)(w1 >> 16))};
+    for (int u = 0; u < D / 64; ++u) {
+      const uint4 k0 = *reinterpret_cast<const uint4*>(cur.k + Stage<D>::k_at(g, 4 * u + c));
+      const uint4 k1 = *reinterpret_cast<const uint4*>(cur.k + Stage<D>::k_at(g + 8, 4 * u + c));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) mma_f16(s[i], f, qf[i][d]);
+      for (int d = 0; d < 4; ++d) {
+        const uint32_t w0 = word(k0, d), w1 = word(k1, d);
+        const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)w0), e4m3x2_to_f16x2((uint16_t)w1),
+                               e4m3x2_to_f16x2((uint16_t)(w0 >> 16)),
+                               e4m3x2_to_f16x2((uint16_t)(w1 >> 16))};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma_f16(s[i], f, qf[i][4 * u + d]);
+      }
     }
 
     // t = S ks rf + log2 vs, masked; a value scale of zero (or below 2^-64) reads as 2^-64
-    float vs[2], lv[2], rv[2];
+    float ks[2], lv[2], rv[2];
+    bool good[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      vs[e] = fmaxf(cur.vs[e], kScaleFloor);
-      lv[e] = __log2f(vs[e]);
-      rv[e] = __frcp_rn(vs[e]);
+      const int t = PAGE16 ? 0 : g + 8 * e;
+      ks[e] = cur.ks[t];
+      good[e] = !(cur.vs[t] < 0.0f);
+      const float vs = fmaxf(cur.vs[t], kScaleFloor);
+      lv[e] = __log2f(vs);
+      rv[e] = __frcp_rn(vs);
     }
-    const bool whole = all_live && t0 >= full_lo && t0 + 16 <= full_hi && good == 0xffffu;
+    const bool whole = __all_sync(0xffffffffu, all_live && t0 >= full_lo && t0 + 16 <= full_hi &&
+                                                   good[0] && good[1]);
     bool passed = false;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float t = fmaf(s[i][e] * rf[i][e & 1], cur.ks[e >> 1], lv[e >> 1]);
+        float t = fmaf(s[i][e] * rf[i][e & 1], ks[e >> 1], lv[e >> 1]);
         if (!whole) {
-          const int tok = g + 8 * (e >> 1), key = t0 + tok;
+          const int key = t0 + g + 8 * (e >> 1);
           const int2 see = mine[i][e & 1];
-          if (!((good >> tok) & 1) || key < max(see.x, lo) || key >= min(see.y, hi)) t = -INFINITY;
+          if (!good[e >> 1] || key < max(see.x, lo) || key >= min(see.y, hi)) t = -INFINITY;
         }
         s[i][e] = t;
         passed |= t > M[i][e & 1] + kLazy;
@@ -308,20 +320,35 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
     }
     // two 16-bit pairs of a word: dims 2j (rows g) and 2j + 1 (rows g + 8) of tokens
     // (2c, 2c+1) and (2c+8, 2c+9)
+    constexpr int kWords = D == 64 ? 2 : 4;  // words of a lane's V row in one read
 #pragma unroll
-    for (int j = 0; j < kMt; ++j) {
-      const int u = D == 64 ? 0 : j / 8, b = D == 64 ? j : j % 8;
-      const uint32_t sel = b % 2 == 0 ? 0x5140 : 0x7362;
-      const uint32_t x = __byte_perm(word(cur.v[0][u], b / 2), word(cur.v[1][u], b / 2), sel);
-      const uint32_t y = __byte_perm(word(cur.v[2][u], b / 2), word(cur.v[3][u], b / 2), sel);
-      const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)x), e4m3x2_to_f16x2((uint16_t)(x >> 16)),
-                             e4m3x2_to_f16x2((uint16_t)y), e4m3x2_to_f16x2((uint16_t)(y >> 16))};
+    for (int u = 0; u < (D == 256 ? 2 : 1); ++u) {
+      uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) mma_f16(o[i][j], f, p[i]);
+      for (int e = 0; e < 4; ++e) {
+        const int t = 2 * c + (e & 1) + 8 * (e >> 1);
+        if constexpr (D == 64) {
+          const uint2 w =
+              *reinterpret_cast<const uint2*>(cur.v + Stage<D>::v_at(t, g >> 1) + 8 * (g & 1));
+          v[e] = make_uint4(w.x, w.y, 0, 0);
+        } else {
+          v[e] = *reinterpret_cast<const uint4*>(cur.v + Stage<D>::v_at(t, 8 * u + g));
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2 * kWords; ++b) {
+        const uint32_t sel = b % 2 == 0 ? 0x5140 : 0x7362;
+        const uint32_t x = __byte_perm(word(v[0], b / 2), word(v[1], b / 2), sel);
+        const uint32_t y = __byte_perm(word(v[2], b / 2), word(v[3], b / 2), sel);
+        const uint32_t f[4] = {e4m3x2_to_f16x2((uint16_t)x), e4m3x2_to_f16x2((uint16_t)(x >> 16)),
+                               e4m3x2_to_f16x2((uint16_t)y), e4m3x2_to_f16x2((uint16_t)(y >> 16))};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma_f16(o[i][8 * u + b], f, p[i]);
+      }
     }
-    cur = nxt;
-    good = good_nxt;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // the ring becomes the place where the warps join
 
   // join the warps
 #pragma unroll
@@ -449,10 +476,14 @@ cudaError_t launch_few(const AttendArgs& a, int64_t most_rows, cudaStream_t stre
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   // whole 16-token steps inside one block need one table entry; other block
   // sizes look each token up
-  if (a.bs % 16 == 0)
-    attend_few_kernel<D, NT, true, T><<<(unsigned)grid, kWarps * 32, 0, stream>>>(a, tiles);
-  else
-    attend_few_kernel<D, NT, false, T><<<(unsigned)grid, kWarps * 32, 0, stream>>>(a, tiles);
+  const auto fn = a.bs % 16 == 0 ? attend_few_kernel<D, NT, true, T> : attend_few_kernel<D, NT, false, T>;
+  const int ring = kWarps * kStages<D> * (int)sizeof(Stage<D>);
+  const int join = kWarps * NT * 8 * (D + 4) * (int)sizeof(float);
+  const int bytes = ring > join ? ring : join;
+  // every call: the attribute belongs to the current device, and setting it is cheap
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  fn<<<(unsigned)grid, kWarps * 32, bytes, stream>>>(a, tiles);
   return cudaGetLastError();
 }
 
@@ -607,7 +638,7 @@ int mshift_attend_block_scaled(
   a.off = paged->off_stride;
   a.head = paged->head_stride;
   a.num_blocks = paged->num_blocks;
-  a.bs = paged->block_size;
+  set_block_size(a, paged->block_size);
   a.ks = k_scale;
   a.vs = v_scale;
   a.ks_blk = ks_blk;

@@ -287,7 +287,7 @@ __device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, i
     if (it >= sp.tiles ||
         (PAGE16 ? (key | 15) < sp.lo || (key & ~15) >= sp.hi : key < sp.lo || key >= sp.hi))
       return -1;
-    const int b = table[key / a.bs];
+    const int b = table[block_column(a, key)];
     if (b >= 0 && b < a.num_blocks) return b;
     flag(a.err, MSHIFT_EBIT_SLOT);
     return -1;
@@ -314,7 +314,7 @@ __device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, i
     for (int i = 0; i < 2; ++i) {
       const int at = first + 64 * i, key = sp.first + it * kTile + at, b = b1[i];
       const float v = fmaxf(vs[i], kScaleFloor);
-      s.at[ring][at] = b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + key % a.bs * a.off : -1ll;
+      s.at[ring][at] = b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + (key - block_column(a, key) * a.bs) * a.off : -1ll;
       s.scale[ring][at] = b >= 0 ? make_float4(ks[i], __log2f(v), __frcp_rn(v), 0.0f)
                                  : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
     }
