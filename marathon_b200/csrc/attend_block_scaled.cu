@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
         a.lse[row * a.hq + i] = -INFINITY;
     }
   }
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be made ready
   // heads fastest: in the NHD layouts neighbouring CTAs read neighbouring bytes
   int64_t id = blockIdx.x;
   const int h = (int)(id % a.hk);
@@ -127,56 +128,6 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
   const int full_lo = max(last.x, lo);                       // keys that every row sees
   const int full_hi = min(a.causal ? head.y : last.y, hi);
   const bool all_live = rq.start + m0 / a.group >= 0;
-
-  // queries: f16 after a power of two for each row
-  uint32_t qf[NT][D / 16][2];
-  float rf[NT][2];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int m = i * 8 + g;
-    float x[D / 4];
-    float top = 0.0f;
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {  // 8 elements of 16 bits
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (m < live) {
-          const T* src = static_cast<const T*>(a.q) + (rq.q0 + (m0 + m) / a.group) * a.q_tok +
-                         (h * a.group + (m0 + m) % a.group) * a.q_head + 64 * u + 16 * c + 8 * p;
-          w = *reinterpret_cast<const uint4*>(src);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Elem<T>::unpack(word(w, e), x + 16 * u + 8 * p + 2 * e);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(x[e]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // exponent of the largest element; rows of zeros, infinities or NaN as they are
-    int e2 = (int)(__float_as_uint(top) >> 23) - 127;
-    if (e2 < -126 || e2 > 126) e2 = 0;
-    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-    const float up = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const float* y = x + 16 * (s / 4) + 4 * (s % 4);
-      qf[i][s][0] = pack_f16x2(y[0] * down, y[1] * down);
-      qf[i][s][1] = pack_f16x2(y[2] * down, y[3] * down);
-    }
-    rf[i][0] = __shfl_sync(0xffffffffu, up, 8 * c);
-    rf[i][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
-  }
-
-  float M[NT][2], l[NT][2], o[NT][kMt][4];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    M[i][0] = M[i][1] = kNoKey;
-    l[i][0] = l[i][1] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kMt; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
-  }
 
   const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
   const uint8_t* kh = a.k + h * a.head;
@@ -233,6 +184,56 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
     fetch(warp + i * kWarps, ahead);
     ahead = block_of(warp + (i + 1) * kWarps);
   }
+  // queries: f16 after a power of two for each row
+  uint32_t qf[NT][D / 16][2];
+  float rf[NT][2];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int m = i * 8 + g;
+    float x[D / 4];
+    float top = 0.0f;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {  // 8 elements of 16 bits
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (m < live) {
+          const T* src = static_cast<const T*>(a.q) + (rq.q0 + (m0 + m) / a.group) * a.q_tok +
+                         (h * a.group + (m0 + m) % a.group) * a.q_head + 64 * u + 16 * c + 8 * p;
+          w = *reinterpret_cast<const uint4*>(src);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Elem<T>::unpack(word(w, e), x + 16 * u + 8 * p + 2 * e);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(x[e]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // exponent of the largest element; rows of zeros, infinities or NaN as they are
+    int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+    if (e2 < -126 || e2 > 126) e2 = 0;
+    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale_log2;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const float* y = x + 16 * (s / 4) + 4 * (s % 4);
+      qf[i][s][0] = pack_f16x2(y[0] * down, y[1] * down);
+      qf[i][s][1] = pack_f16x2(y[2] * down, y[3] * down);
+    }
+    rf[i][0] = __shfl_sync(0xffffffffu, up, 8 * c);
+    rf[i][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+  }
+
+  float M[NT][2], l[NT][2], o[NT][kMt][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    M[i][0] = M[i][1] = kNoKey;
+    l[i][0] = l[i][1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+  }
+
 #pragma unroll 1
   for (int st = warp; st < steps; st += kWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kS - 2) : "memory");
@@ -406,66 +407,100 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
   }
 }
 
-// o = sum_s 2^(M_s - M) acc_s / sum_s 2^(M_s - M) l_s over the splits of one (row, head);
-// a CTA for each, a thread for each dim.  ROWS: of the many-rows kernel.
-template <int D, typename T, bool ROWS>
-__global__ void __launch_bounds__(D) attend_join_kernel(const AttendArgs a) {
-  extern __shared__ float s_by[];
-  __shared__ float s_red[2][D / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// o = sum_s 2^(M_s - M) acc_s / sum_s 2^(M_s - M) l_s over the splits of one (row, head), which WPR
+// warps share: one where there are few splits (a chunk's many rows), eight where a few rows
+// have many (decoding over a long cache).  ROWS: of the many-rows kernel.
+constexpr int kJoinWarps = 8;
+template <int D, typename T, bool ROWS, int WPR>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs a, int64_t total) {
+  constexpr int kVec = D / 32;  // dims of a lane
+  constexpr unsigned kAll = 0xffffffffu;
+  __shared__ float s_x[WPR > 1 ? kJoinWarps : 1][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part_of = warp % WPR;
   const int chunk = ROWS ? a.rchunk : a.chunk, nsplit = ROWS ? a.rsplit : a.nsplit;
-  const float* part_o = ROWS ? a.rpart_o : a.part_o;
-  const float2* part_ml = ROWS ? a.rpart_ml : a.part_ml;
+  const int64_t id = (int64_t)blockIdx.x * (kJoinWarps / WPR) + warp / WPR;
+  int64_t row = -1;
+  int hq = 0;
+  Request rq{};
+  if (id < total) {
+    if (!ROWS && a.cap) {
+      const int64_t m = id % a.cap, rh = id / a.cap;
+      rq = request_of(a, (int)(rh / a.hk), false);
+      if (m < (int64_t)rq.n * a.group) row = rq.q0 + m / a.group;
+      hq = (int)(rh % a.hk) * a.group + (int)(m % a.group);
+    } else if (id / a.hq < row_start(a.qs, a.reqs, a.rows)) {
+      row = id / a.hq;
+      hq = (int)(id % a.hq);
+      const int r =
+          find_request(a.reqs, row, [&](int i) { return (long long)row_start(a.qs, i, a.rows); });
+      rq = request_of(a, r, false);
+      if (row < rq.q0 || row >= rq.q0 + rq.n) row = -1;
+    }
+    if (((int64_t)rq.n * a.group > a.few_rows) != ROWS) row = -1;
+  }
+  // nothing the kernel before wrote has been read so far
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int64_t row;
-  int hq;
-  Request rq;
-  if (!ROWS && a.cap) {
-    const int64_t m = blockIdx.x % a.cap, rh = blockIdx.x / a.cap;
-    const int r = (int)(rh / a.hk);
-    rq = request_of(a, r, false);
-    if (m >= (int64_t)rq.n * a.group) return;
-    row = rq.q0 + m / a.group;
-    hq = (int)(rh % a.hk) * a.group + (int)(m % a.group);
-  } else {
-    row = blockIdx.x / a.hq;
-    hq = blockIdx.x % a.hq;
-    if (row >= row_start(a.qs, a.reqs, a.rows)) return;
-    const int r =
-        find_request(a.reqs, row, [&](int i) { return (long long)row_start(a.qs, i, a.rows); });
-    rq = request_of(a, r, false);
-    if (row < rq.q0 || row >= rq.q0 + rq.n) return;
-  }
-  if (((int64_t)rq.n * a.group > a.few_rows) != ROWS) return;
-  const int2 see = seen(a, rq, rq.start + (row - rq.q0));
+  if (WPR == 1 && row < 0) return;  // else the row's warps, all alike, still meet below
+
+  const int2 see = row < 0 ? make_int2(0, 0) : seen(a, rq, rq.start + (row - rq.q0));
   // splits that hold a key of this row; at least one, for a row without keys
-  const int s0 = see.x / chunk, s1 = max((see.y + chunk - 1) / chunk, s0 + 1);
-  const int64_t part = blockIdx.x * (int64_t)nsplit;
+  const int s0 = see.x / chunk, s1 = row < 0 ? s0 : max((see.y + chunk - 1) / chunk, s0 + 1);
+  const int64_t part = id * nsplit;
+  const float2* ml = (ROWS ? a.rpart_ml : a.part_ml) + part;
+  const float* acc = (ROWS ? a.rpart_o : a.part_o) + part * D + lane * kVec;
   float top = kNoKey;
-  for (int s = s0 + tid; s < s1; s += D) top = fmaxf(top, part_ml[part + s].x);
-  for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (lane == 0) s_red[0][warp] = top;
-  __syncthreads();
-  for (int w = 0; w < D / 32; ++w) top = fmaxf(top, s_red[0][w]);
+  for (int s = s0 + lane; s < s1; s += 32) top = fmaxf(top, ml[s].x);
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
   float sum = 0.0f;
-  for (int s = s0 + tid; s < s1; s += D) {
-    const float2 ml = part_ml[part + s];
-    const float by = ex2(ml.x - top);
-    s_by[s - s0] = by;
-    sum = fmaf(ml.y, by, sum);
+  for (int s = s0 + lane; s < s1; s += 32) {
+    const float2 y = ml[s];
+    sum = fmaf(y.y, ex2(y.x - top), sum);
   }
-  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) s_red[1][warp] = sum;
-  __syncthreads();
-  sum = 0.0f;
-  for (int w = 0; w < D / 32; ++w) sum += s_red[1][w];
-  float x = 0.0f;
-  const float* src = part_o + (part + s0) * D + tid;
-#pragma unroll 8
-  for (int s = 0; s < s1 - s0; ++s) x = fmaf(src[(int64_t)s * D], s_by[s], x);
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(kAll, sum, d);
+  float x[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) x[e] = 0.0f;
+#pragma unroll 4
+  for (int s = s0 + part_of; s < s1; s += WPR) {
+    const float by = ex2(ml[s].x - top);
+    const float* y = acc + (int64_t)s * D;
+    float f[kVec];
+    if constexpr (kVec == 2) {
+      const float2 z = *reinterpret_cast<const float2*>(y);
+      f[0] = z.x;
+      f[1] = z.y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; e += 4) {
+        const float4 z = *reinterpret_cast<const float4*>(y + e);
+        f[e] = z.x;
+        f[e + 1] = z.y;
+        f[e + 2] = z.z;
+        f[e + 3] = z.w;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = fmaf(f[e], by, x[e]);
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) s_x[warp][lane * kVec + e] = x[e];
+    __syncthreads();
+    if (part_of > 0 || row < 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[e] += s_x[warp + w][lane * kVec + e];
+  }
   const bool any = top > kNoKey;
-  static_cast<T*>(a.out)[row * a.o_tok + hq * a.o_head + tid] = Elem<T>::put(any ? x / sum : 0.0f);
-  if (tid == 0 && a.lse != nullptr)
+  T* dst = static_cast<T*>(a.out) + row * a.o_tok + hq * a.o_head + lane * kVec;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) x[e] = any ? x[e] / sum : 0.0f;
+#pragma unroll
+  for (int e = 0; e < kVec; e += 2) reinterpret_cast<uint32_t*>(dst)[e / 2] = Elem<T>::pack(x + e);
+  if (lane == 0 && a.lse != nullptr)
     a.lse[row * a.hq + hq] = any ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
@@ -489,19 +524,23 @@ cudaError_t launch_few(const AttendArgs& a, int64_t most_rows, cudaStream_t stre
 
 template <int D, typename T, bool ROWS>
 cudaError_t launch_join(const AttendArgs& a, cudaStream_t stream) {
-  const int64_t grid = !ROWS && a.cap ? (int64_t)a.reqs * a.hk * a.cap : (int64_t)a.rows * a.hq;
+  const int64_t total = !ROWS && a.cap ? (int64_t)a.reqs * a.hk * a.cap : (int64_t)a.rows * a.hq;
+  // a warp a row while that is one round of reads, or where the rows alone fill the GPU
+  const int nsplit = ROWS ? a.rsplit : a.nsplit;
+  const bool one = nsplit <= 4 || total >= 148 * 64;
+  const int64_t grid = one ? (total + kJoinWarps - 1) / kJoinWarps : total;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(D);
-  cfg.dynamicSmemBytes = sizeof(float) * (ROWS ? a.rsplit : a.nsplit);
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T, ROWS>, a);
+  return one ? cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T, ROWS, 1>, a, total)
+             : cudaLaunchKernelEx(&cfg, attend_join_kernel<D, T, ROWS, kJoinWarps>, a, total);
 }
 
 template <int D, typename T>
@@ -563,7 +602,7 @@ Plan plan(int32_t rows, int32_t hq, int32_t hk, int32_t head_size, int32_t reqs,
   p.few_rows = head_size > 128 ? INT32_MAX : kFewRows;
   const int64_t few = all < p.few_rows ? all : p.few_rows;
   const int64_t tiles = few <= 8 ? 1 : (few + 15) / 16;
-  p.chunk = chunk_for((int64_t)reqs * hk * tiles, 148 * 8, max_len, 256, 2048);
+  p.chunk = chunk_for((int64_t)reqs * hk * tiles, 148 * 4, max_len, 256, 4096);
   p.nsplit = max_len > 0 ? (int)(((int64_t)max_len + p.chunk - 1) / p.chunk) : 1;
   p.cap = (int64_t)reqs * hk * few <= (int64_t)rows * hq ? few : 0;
   if (p.nsplit > 1) p.parts = (p.cap ? (int64_t)reqs * hk * p.cap : (int64_t)rows * hq) * p.nsplit;
