@@ -9,10 +9,11 @@
 // end moves by up to one binade) and makes division, growth and the attention's
 // dequantisation exact but for codes that fall below 2^-6 * new.
 //
-// Bound by HBM: each row is read once, each code written once.  One warp has
-// one (block, head, side): it keeps a block's rows in registers between the
-// maximum and the rounding, so nothing is read twice for blocks of 16 tokens of
-// up to 512 bytes a row; longer blocks are walked twice, the second time from L2.
+// Bound by HBM: each row is read once, each code written once.  One warp has one (block,
+// head), K and V: it keeps the block's rows in registers between the maximum and the rounding, so
+// nothing is read twice for blocks of 16 tokens of up to 512 bytes a row; longer blocks
+// are walked twice, the second time from L2.  Both sides' loads are issued before either is used, since
+// what comes before them (the request, its length, its table) is a chain of dependent reads.
 // Heads are neighbouring warps, which makes a CTA's reads and writes whole rows of
 // the NHD layout.  No atomics, no workspace: a block's tokens are consecutive rows
 // of one request, so the warp sees all of them.
@@ -79,8 +80,7 @@ __global__ void __launch_bounds__(kAppWarps * 32) append_kernel(const AppArgs a)
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kAppWarps + (threadIdx.x >> 5);
   const int h = (int)(w % a.heads);
-  const int side = (int)((w / a.heads) & 1);
-  const int64_t item = w / (2 * a.heads);
+  const int64_t item = w / a.heads;
   if (item >= a.items) return;
 
   // a request of n tokens touches at most n / bs + 2 blocks, and
@@ -105,18 +105,13 @@ __global__ void __launch_bounds__(kAppWarps * 32) append_kernel(const AppArgs a)
     return;
   }
 
-  const T* src = static_cast<const T*>(side ? a.v : a.k);
-  const int64_t tok = side ? a.v_tok : a.k_tok;
-  src += (q0 + (lo - start)) * tok + h * (side ? a.v_head : a.k_head);
-  uint8_t* page = (side ? a.vc : a.kc) + block * a.blk + h * a.head;
-  float* scale = side ? a.vs + block * a.vs_blk + h * a.vs_head
-                      : a.ks + block * a.ks_blk + h * a.ks_head;
   const int count = (int)(hi - lo), off0 = (int)(lo - col * a.bs);
   const int sub = lane / kLanes, part = (lane % kLanes) * kPerLane;  // row of the load, place in it
+  const T* k_src = static_cast<const T*>(a.k) + (q0 + (lo - start)) * a.k_tok + h * a.k_head;
+  const T* v_src = static_cast<const T*>(a.v) + (q0 + (lo - start)) * a.v_tok + h * a.v_head;
+  const int64_t page = block * a.blk + h * a.head;
 
-  uint4 keep[kKeep];
-  float amax = 0.0f;
-  auto load = [&](int row0) {
+  auto load = [&](uint4* keep, const T* src, int64_t tok, int row0) {
 #pragma unroll
     for (int i = 0; i < kKeep; ++i) {
       const int row = row0 + (i / kPerLane) * kRows + sub;
@@ -125,73 +120,145 @@ __global__ void __launch_bounds__(kAppWarps * 32) append_kernel(const AppArgs a)
         keep[i] = *reinterpret_cast<const uint4*>(src + row * tok + (part + i % kPerLane) * kVec);
     }
   };
-  for (int row0 = 0; row0 < count; row0 += kChunk) {
-    load(row0);
+  // Largest magnitude as its bits, which order as the values do: both halves of a word of 16-bit
+  // elements at once.
+  auto largest = [&](const uint4* keep, uint32_t top) {
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+      const uint32_t w[4] = {keep[i].x, keep[i].y, keep[i].z, keep[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        top = kVec == 8 ? __vmaxu2(top, w[e] & 0x7fff7fffu) : max(top, w[e] & 0x7fffffffu);
+    }
+    return top;
+  };
+  // The same without infinities and NaN, for rows that have some.
+  auto largest_finite = [&](const T* src, int64_t tok) {
+    float amax = 0.0f;
+#pragma unroll 1
+    for (int i = lane; i < count * D; i += 32) {
+      const float m = fabsf(Elem<T>::get(src[i / D * tok + i % D]));
+      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    return amax;
+  };
+  // The block's new scale; earlier codes follow it.
+  auto rescale = [&](uint8_t* rows, float* scale, uint32_t top, const T* src, int64_t tok) {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, top, d);
+      top = kVec == 8 ? __vmaxu2(top, o) : max(top, o);
+    }
+    if (kVec == 8) top = __vmaxu2(top, top >> 16) & 0xffffu;
+    float f[2];
+    Elem<T>::unpack(top, f);
+    const float amax = f[0] <= 3.402823466e38f ? f[0] : largest_finite(src, tok);
+    float s = scale_for(amax);
+    if (off0 > 0) {  // the block holds earlier tokens of the request
+      const float old = *scale;
+      s = fmaxf(old, s);
+      if (s != old) {
+        const float ratio = old / s;
+        constexpr int kWords = D / 4;
+#pragma unroll 1
+        for (int i = lane; i < off0 * kWords; i += 32) {
+          uint32_t* p = reinterpret_cast<uint32_t*>(rows + (i / kWords) * a.off) + i % kWords;
+          const uint32_t c = *p;
+          const uint32_t lo2 = e4m3x2_to_f16x2((uint16_t)c);
+          const uint32_t hi2 = e4m3x2_to_f16x2((uint16_t)(c >> 16));
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo2));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi2));
+          *p = f32x2_to_e4m3x2(x.x * ratio, x.y * ratio) |
+               ((uint32_t)f32x2_to_e4m3x2(y.x * ratio, y.y * ratio) << 16);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the old scale
+    if (lane == 0) *scale = s;
+    return s;
+  };
+  auto store = [&](const uint4* keep, uint8_t* rows, float s, int row0) {
+    // x / s: the scales written here are powers of two, whose reciprocal is exact
+    const float inv = 1.0f / s;
+    uint8_t* to = rows + (off0 + row0 + sub) * a.off + part * kVec;
 #pragma unroll
     for (int i = 0; i < kKeep; ++i) {
       float f[kVec];
       unpack16<T>(keep[i], f);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const float m = fabsf(f[e]);
-        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // not infinities, not NaN
-      }
-    }
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-  float s = scale_for(amax);
-  if (off0 > 0) {  // the block holds earlier tokens of the request
-    const float old = *scale;
-    s = fmaxf(old, s);
-    if (s != old) {
-      const float ratio = old / s;
-      constexpr int kWords = D / 4;
-      for (int i = lane; i < off0 * kWords; i += 32) {
-        uint32_t* p = reinterpret_cast<uint32_t*>(page + (i / kWords) * a.off) + i % kWords;
-        const uint32_t c = *p;
-        const uint32_t lo2 = e4m3x2_to_f16x2((uint16_t)c), hi2 = e4m3x2_to_f16x2((uint16_t)(c >> 16));
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo2));
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi2));
-        *p = f32x2_to_e4m3x2(x.x * ratio, x.y * ratio) |
-             ((uint32_t)f32x2_to_e4m3x2(y.x * ratio, y.y * ratio) << 16);
-      }
-    }
-  }
-  if (lane == 0) *scale = s;
-
-  // x / s: the scales written here are powers of two, whose reciprocal is exact;
-  // a scale of another origin takes the division
-  const bool pow2 = (__float_as_uint(s) & 0x7fffffu) == 0;
-  const float inv = 1.0f / s;
-  for (int row0 = 0; row0 < count; row0 += kChunk) {
-    if (count > kChunk) load(row0);
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-      const int row = row0 + (i / kPerLane) * kRows + sub;
-      if (row >= count) continue;
-      float f[kVec];
-      unpack16<T>(keep[i], f);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) f[e] = pow2 ? f[e] * inv : f[e] / s;
       uint32_t o[kVec / 4];
 #pragma unroll
       for (int e = 0; e < kVec / 4; ++e)
-        o[e] = f32x2_to_e4m3x2(f[4 * e], f[4 * e + 1]) |
-               ((uint32_t)f32x2_to_e4m3x2(f[4 * e + 2], f[4 * e + 3]) << 16);
-      uint32_t* p = reinterpret_cast<uint32_t*>(page + (off0 + row) * a.off +
-                                                (part + i % kPerLane) * kVec);
-      if constexpr (kVec == 8)
-        *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
-      else
-        *p = o[0];
+        o[e] = f32x2_to_e4m3x2(f[4 * e] * inv, f[4 * e + 1] * inv) |
+               ((uint32_t)f32x2_to_e4m3x2(f[4 * e + 2] * inv, f[4 * e + 3] * inv) << 16);
+      if (row0 + (i / kPerLane) * kRows + sub < count) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(to + (i / kPerLane) * kRows * a.off + i % kPerLane * kVec);
+        if constexpr (kVec == 8)
+          *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
+        else
+          *p = o[0];
+      }
+    }
+  };
+  // A scale of another origin, kept because it is large enough, takes the division.
+  auto store_divided = [&](const T* src, int64_t tok, uint8_t* rows, float s) {
+#pragma unroll 1
+    for (int i = lane; i < count * (D / 2); i += 32) {
+      const T* x = src + i / (D / 2) * tok + i % (D / 2) * 2;
+      *reinterpret_cast<uint16_t*>(rows + (off0 + i / (D / 2)) * a.off + i % (D / 2) * 2) =
+          f32x2_to_e4m3x2(Elem<T>::get(x[0]) / s, Elem<T>::get(x[1]) / s);
+    }
+  };
+  auto power_of_two = [](float s) { return (__float_as_uint(s) & 0x7fffffu) == 0; };
+
+  float* k_scale = a.ks + block * a.ks_blk + h * a.ks_head;
+  float* v_scale = a.vs + block * a.vs_blk + h * a.vs_head;
+  uint8_t *k_rows = a.kc + page, *v_rows = a.vc + page;
+  if (count <= kChunk) {
+    uint4 kk[kKeep], vv[kKeep];
+    load(kk, k_src, a.k_tok, 0);
+    load(vv, v_src, a.v_tok, 0);
+    const float ks = rescale(k_rows, k_scale, largest(kk, 0), k_src, a.k_tok);
+    if (power_of_two(ks))
+      store(kk, k_rows, ks, 0);
+    else
+      store_divided(k_src, a.k_tok, k_rows, ks);
+    const float vs = rescale(v_rows, v_scale, largest(vv, 0), v_src, a.v_tok);
+    if (power_of_two(vs))
+      store(vv, v_rows, vs, 0);
+    else
+      store_divided(v_src, a.v_tok, v_rows, vs);
+    return;
+  }
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const T* src = side ? v_src : k_src;
+    const int64_t tok = side ? a.v_tok : a.k_tok;
+    uint8_t* rows = side ? v_rows : k_rows;
+    uint4 keep[kKeep];
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int row0 = 0; row0 < count; row0 += kChunk) {
+      load(keep, src, tok, row0);
+      top = largest(keep, top);
+    }
+    const float s = rescale(rows, side ? v_scale : k_scale, top, src, tok);
+    if (!power_of_two(s)) {
+      store_divided(src, tok, rows, s);
+      continue;
+    }
+#pragma unroll 1
+    for (int row0 = 0; row0 < count; row0 += kChunk) {
+      load(keep, src, tok, row0);
+      store(keep, rows, s, row0);
     }
   }
 }
 
 template <typename T>
 int launch_append(const AppArgs& a, int head_size, cudaStream_t stream) {
-  const int64_t warps = a.items * 2 * a.heads;
+  const int64_t warps = a.items * a.heads;
   const int64_t grid = (warps + kAppWarps - 1) / kAppWarps;
   if (grid > INT32_MAX) return MSHIFT_EINVAL;
   const dim3 g((unsigned)grid), b(kAppWarps * 32);
