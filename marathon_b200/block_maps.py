@@ -76,10 +76,10 @@ def block_maps(
         if at < end and table < at + 4 * n:
             raise _lib.ShiftError("an argument shares memory with block_tables, which are written")
     query_start = cached_lens.new_empty(reqs + 1)
-    seq_lens = cached_lens.new_empty(reqs)
-    head = cached_lens.new_empty(1)
+    seq_lens = torch.empty_like(cached_lens)
+    head = torch.empty_like(free_head)
     slots = cached_lens.new_empty(tokens, dtype=torch.int64)
-    positions = cached_lens.new_empty(tokens, dtype=torch.int64)
+    positions = torch.empty_like(slots)
     launch(_lib.load().mshift_block_maps, "block_maps", dev, (
         read[0], read[1], reqs, table, stride, width, read[2], n_free, read[3], block_size, tokens,
         query_start.data_ptr(), seq_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),

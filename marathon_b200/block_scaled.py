@@ -178,7 +178,10 @@ def attend_block_scaled(
     zero_tail = out is None
     if zero_tail:
         # the kernels write every row, unless there is no request and so no kernel
-        out = q.new_empty((rows, hq, head_size)) if reqs else q.new_zeros((rows, hq, head_size))
+        if not reqs:
+            out = q.new_zeros((rows, hq, head_size))
+        else:
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, hq, head_size))
         o_tok, o_head = hq * head_size, head_size
         if return_lse:
             lse = q.new_empty((rows, hq), dtype=torch.float32)

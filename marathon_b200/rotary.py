@@ -120,10 +120,10 @@ def rotary_axes(
     else:
         q_out = q_to = k_out = k_to = None
         if q is not None:
-            q_out = q.new_empty(shape)
+            q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
             q_to = (q_out.data_ptr(), hq * head_size, head_size)
         if k is not None:
-            k_out = k.new_empty(k.shape)
+            k_out = torch.empty_like(k) if k.is_contiguous() else k.new_empty(k.shape)
             k_to = (k_out.data_ptr(), hk * head_size, head_size)
     launch(_lib.load().mshift_rotary_axes, "rotary_axes", dev, (
         code, *q_in, *(q_to or q_in), hq, *k_in, *(k_to or k_in), hk, n, head_size, 2 * half,
