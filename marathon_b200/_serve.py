@@ -136,6 +136,8 @@ def _status_word(index: int) -> int:
 def launch(fn, what: str, device: int, args: tuple, check: bool) -> None:
     """Call the entry point with the device's status word and current stream behind ``args``,
     that device being current."""
+    if check and torch.cuda.is_current_stream_capturing():
+        raise ShiftError(f"{what}: check=True waits for the device and cannot be captured")
     err = _status.get(device) or _status_word(device)
     stream = torch._C._cuda_getCurrentRawStream(device)
     if torch.cuda.current_device() == device:

@@ -88,9 +88,11 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  if (a.zero_tail) {  // rows behind the last request
-    for (int64_t row = row_start(a.qs, a.reqs, a.rows) + (int64_t)blockIdx.x; row < a.rows;
-         row += gridDim.x) {
+  if (a.zero_tail) {  // rows of no request
+    const int before = row_start(a.qs, 0, a.rows), behind = row_start(a.qs, a.reqs, a.rows);
+    const int64_t none = before + (int64_t)a.rows - behind;
+    for (int64_t i0 = blockIdx.x; i0 < none; i0 += gridDim.x) {
+      const int64_t row = i0 < before ? i0 : i0 - before + behind;
       for (int i = threadIdx.x; i < a.hq * D; i += kWarps * 32)
         static_cast<T*>(a.out)[row * a.o_tok + (i / D) * a.o_head + i % D] = Elem<T>::put(0.0f);
       for (int i = threadIdx.x; i < a.hq && a.lse != nullptr; i += kWarps * 32)
@@ -506,7 +508,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 
 template <int D, int NT, typename T>
 cudaError_t launch_few(const AttendArgs& a, int64_t most_rows, cudaStream_t stream) {
-  const int tiles = (int)((most_rows + NT * 8 - 1) / (NT * 8));
+  // at least one, for the rows of no request
+  const int tiles = most_rows > 0 ? (int)((most_rows + NT * 8 - 1) / (NT * 8)) : 1;
   const int64_t grid = (int64_t)a.reqs * a.nsplit * tiles * a.hk;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   // whole 16-token steps inside one block need one table entry; other block
@@ -657,7 +660,7 @@ int mshift_attend_block_scaled(
       seq_lens == nullptr || out == nullptr || err == nullptr)
     return MSHIFT_EINVAL;
   const auto odd = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
-  if (odd(q) || odd(k_base) || odd(v_base) || q_tok % 8 || q_head % 8 || paged->blk_stride % 16 ||
+  if (odd(q) || odd(out) || odd(k_base) || odd(v_base) || o_tok % 8 || o_head % 8 || q_tok % 8 || q_head % 8 || paged->blk_stride % 16 ||
       paged->off_stride % 16 || paged->head_stride % 16)
     return MSHIFT_EINVAL;
   const Plan p = plan(rows, hq, paged->heads, paged->head_size, reqs, max_query_len, max_seq_len);

@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kTile = 128;  // keys of a tile, rows of a row tile
 constexpr int kHalf = 64;   // keys whose scores a softmax thread holds at once
+constexpr int kByHand = 4;  // of 16 exponentials, those that the FMA units work out
 constexpr int kCta = 512;
 constexpr int kRing = 4;  // tiles whose places and scales are held
 constexpr uint32_t kRounds = 1u << 18;  // try_wait rounds of a wait
@@ -199,6 +200,31 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^x of a pair without the special-function unit: x = n + f with n the nearest whole number (from
+// adding 1.5 * 2^23, whose low bits then hold n), 2^f by a polynomial of degree 5 fitted here for the
+// least relative error on [-1/2, 1/2] (7.5e-8, 2.3e-7 with fp32's rounding), and n added to its
+// exponent.  Below -126, masked keys' -inf among it, the result is 2^-126, which f16 rounds to zero;
+// NaN stays NaN.
+__device__ __forceinline__ float2 exp2_pair(float x0, float x1) {
+  constexpr float kMagic = 12582912.0f;
+  const uint64_t x = pair(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
+  const uint64_t t = add2(x, pair(kMagic, kMagic));
+  const uint64_t f = add2(x, fma2(t, pair(-1.0f, -1.0f), pair(kMagic, kMagic)));
+  uint64_t r = fma2(f, pair(0x1.5c08e2p-10f, 0x1.5c08e2p-10f), pair(0x1.3d0c54p-7f, 0x1.3d0c54p-7f));
+  r = fma2(r, f, pair(0x1.c6b6e6p-5f, 0x1.c6b6e6p-5f));
+  r = fma2(r, f, pair(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+  r = fma2(r, f, pair(0x1.62e428p-1f, 0x1.62e428p-1f));
+  r = fma2(r, f, pair(0x1.000002p+0f, 0x1.000002p+0f));
+  const float2 y = unpair(r), n = unpair(t);
+  return unpair(fma2(x, pair(0.0f, 0.0f),
+                     pair(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                          __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)))));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -596,7 +622,15 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
         uint64_t sum = 0;
 #pragma unroll
         for (int e = c; e < c + 16; e += 2) {
-          const float p0 = ex2(__uint_as_float(x[e])), p1 = ex2(__uint_as_float(x[e + 1]));
+          float p0, p1;
+          if (e % 16 >= 16 - kByHand) {
+            const float2 z = exp2_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            p0 = z.x;
+            p1 = z.y;
+          } else {
+            p0 = ex2(__uint_as_float(x[e]));
+            p1 = ex2(__uint_as_float(x[e + 1]));
+          }
           if constexpr (PAGE16)
             sum = add2(sum, pair(p0, p1));
           else

@@ -355,6 +355,70 @@ def test_rows_behind_the_last_request(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,new,hq,hk,d,bs,layout,window", [
+    ([2500], [300], 4, 1, 128, 16, "nhd", 0),
+    ([3300, 700, 20], [90, 513, 1], 10, 2, 64, 32, "split", 0),
+    ([1900], [1900], 1, 1, 128, 16, "hnd", 300),
+    ([1500, 40], [77, 40], 6, 2, 128, 24, "nhd", 0),
+    ([2048, 2049], [64, 65], 2, 1, 64, 128, "split_blocks", 0),
+    ([1100], [130], 5, 1, 256, 16, "nhd", 0),
+])
+def test_many_rows_over_many_key_tiles(cuda, lens, new, hq, hk, d, bs, layout, window):
+    """Longer than every ring of stages, with and without splits of the keys."""
+    c = Case(cuda, lens, new, hq, hk, d, bs, layout, seed=len(lens))
+    c.check(c.run(window=window), window=window)
+    c.check(c.run(window=window, max_seq_len=60000), window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 60])
+def test_nan_keys_reach_the_rows_that_see_them_and_no_others(cuda, new):
+    """Every place of a step in turn, so that each way an exponential is worked out meets one."""
+    at = 130
+    c = Case(cuda, [200, 150], [new, new], 4, 2, 128, 16, seed=5)
+    good = c.run()
+    for key in range(at, at + 18):
+        kv = c.dev[1].clone()
+        block = c.tables[0][key // 16]
+        kv.view(torch.uint8)[block, key % 16, 1, 7] = NAN_CODE
+        out, lse = attend_block_scaled(c.dev[0], kv, *c.dev[2:], *c.step, 16, "nhd", return_lse=True,
+                                       check=True, **c.bounds)
+        row = torch.arange(2 * new, device=cuda)
+        hit = (row < new) & (200 - new + row >= key)
+        assert bool(lse[hit][:, 2:].isnan().all()) and bool(out[hit][:, 2:].isnan().all())
+        assert torch.equal(out[~hit], good[0][~hit]) and torch.equal(lse[~hit], good[1][~hit])
+        assert torch.equal(out[:, :2], good[0][:, :2])
+
+
+@pytest.mark.gpu
+def test_empty_steps_and_rows_before_the_first_request(cuda):
+    c = Case(cuda, [40, 9], [0, 0], 4, 2, 128, 16, pad=5)
+    for bound in (40, 40000):
+        out, lse = c.run(max_query_len=0, max_seq_len=bound)
+        assert bool((out == 0).all()) and bool((lse == float("-inf")).all())
+    c = Case(cuda, [40], [3], 4, 2, 128, 16, pad=5)
+    want, _ = c.run()
+    c.step[1] = _i32(cuda, [2, 5])
+    c.dev[0] = c.dev[0].roll(2, 0)
+    out, lse = c.run()
+    assert torch.equal(out[2:5], want[:3]) and bool((out[:2] == 0).all()) and bool((out[5:] == 0).all())
+    assert bool((lse[:2] == float("-inf")).all())
+
+
+@pytest.mark.gpu
+def test_check_cannot_be_captured(cuda):
+    c = Case(cuda, [40], [1], 4, 2, 128, 16)
+    c.run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = attend_block_scaled(*c.dev, *c.step, 16, "nhd", **c.bounds)
+        with pytest.raises(ShiftError, match="captured"):
+            c.run()
+    g.replay()
+    assert torch.equal(out, c.run()[0])
+
+
+@pytest.mark.gpu
 def test_strided_queries_outputs_and_scales(cuda):
     c = Case(cuda, [60, 200], [3, 70], 4, 2, 128, 16, seed=6)
     want, wl = c.run()
