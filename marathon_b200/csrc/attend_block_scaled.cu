@@ -592,6 +592,28 @@ int chunk_for(int64_t units, int64_t want, int max_len, int64_t least, int64_t m
   return (int)((chunk + 127) / 128 * 128);
 }
 
+// Keys of a split of the many-rows kernel.  One CTA an SM: `units` CTAs a split run in rounds of
+// 148, each as long as its tiles of 128 keys and five more for starting and writing back (a tile takes
+// 2.3 us, both measured).  Splitting fills the last round, and costs the partial results' way to memory and
+// back and the join's launch; the cheapest count is taken.  Measured both ways: 64-244 tokens over eight
+// histories 483 us whole, 506 in three, 457 in four; 1,024 tokens over 16,384 297 us whole, 370 in seven; 244
+// over 30,720 654 us whole, 250-260 in seven to fifteen.
+int rows_chunk(int64_t units, int max_len, int64_t elements) {
+  const int64_t tiles = ((int64_t)max_len + 127) / 128;
+  const double part = (double)elements * 8 / 6.5e12 / 2.3e-6;  // of a split, in tiles
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t s = 1; s <= 64 && (s == 1 || tiles / s >= 8); ++s) {
+    const double rounds = (double)((units * s + 147) / 148);
+    const double cost = rounds * ((double)((tiles + s - 1) / s) + 5.0) + (s > 1 ? (double)s * part + 3.0 : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best == 1 ? 1 << 30 : (int)((tiles + best - 1) / best * 128);
+}
+
 struct Plan {
   int few_rows, chunk, nsplit, rchunk, rsplit;
   int64_t cap;
@@ -613,7 +635,7 @@ Plan plan(int32_t rows, int32_t hq, int32_t hk, int32_t head_size, int32_t reqs,
   p.rsplit = 1;
   if (all > p.few_rows) {
     const int64_t items = (int64_t)rows * group / 256 + reqs;
-    p.rchunk = chunk_for(items * hk, 148 * 4, max_len, 1024, 1 << 30);
+    p.rchunk = rows_chunk(items * hk, max_len, (int64_t)rows * hq * head_size);
     p.rsplit = max_len > 0 ? (int)(((int64_t)max_len + p.rchunk - 1) / p.rchunk) : 1;
     if (p.rsplit > 1) p.rparts = (int64_t)rows * hq * p.rsplit;
   }
