@@ -143,8 +143,9 @@ def attend_block_scaled(
     ``-inf``.  Rows behind the last request are left as they were in a given ``out``, and
     zeros (lse ``-inf``) otherwise.  Keys at positions that no row of a tile of rows may see are not
     read, so stale codes there do no harm, NaN included; a NaN among the values of a token that later rows of the
-    same request see can reach its earlier rows too.  Value scales must be positive (below 2^-64 they are read
-    as 2^-64).
+    same request see can reach its earlier rows too.  Rows past ``max_query_len`` are not written.
+    Value scales must be positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of
+    each other.
 
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
     the bounds (cut off there), positions past the block table (unseen).

