@@ -467,6 +467,29 @@ def test_cache_with_gaps_between_blocks_and_past_32_bits(cuda):
 
 
 @pytest.mark.gpu
+def test_append_and_many_rows_in_blocks_past_32_bits(cuda):
+    """Blocks 2.5 GB apart, so that the third starts past 2^32 bytes."""
+    heads, d, bs, stride = 2, 64, 16, 5 * 2**29
+    buf = torch.zeros(2 * stride + bs * heads * 2 * d, dtype=torch.uint8, device=cuda)
+    kv = buf.as_strided((3, bs, heads, 2 * d), (stride, heads * 2 * d, 2 * d, 1)).view(F8)
+    ks, vs = (torch.ones(3, heads, device=cuda) for _ in range(2))
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(30, heads, d, generator=g).bfloat16() for _ in range(2))
+    step = [_i32(cuda, [[0, 2]]), _i32(cuda, [0, 30]), _i32(cuda, [30])]
+    append_block_scaled(k.to(cuda), v.to(cuda), kv, ks, vs, *step, bs, check=True)
+    want = torch.zeros(3, bs, heads, 2 * d, dtype=torch.float64)
+    wks, wvs = (torch.ones(3, heads, dtype=torch.float64) for _ in range(2))
+    serving.append(k, v, want, wks, wvs, [[0, 2]], [0, 30], [30], bs, "nhd")
+    for b in range(3):
+        assert torch.equal(kv[b].cpu().double(), want[b])
+    assert torch.equal(ks.cpu().double(), wks) and torch.equal(vs.cpu().double(), wvs)
+    c = Case(cuda, [30], [30], 4, heads, d, bs)
+    c.kv, c.ks, c.vs, c.tables = torch.stack([kv[b].cpu() for b in range(3)]), wks, wvs, [[0, 2]]
+    c.dev, c.step = [c.dev[0], kv, ks, vs], step
+    c.check(c.run())
+
+
+@pytest.mark.gpu
 def test_bad_blocks_lengths_and_bounds_are_flagged(cuda):
     take_errors(cuda)
     c = Case(cuda, [64, 64], [1, 20], 4, 2, 128, 16, seed=1)
