@@ -169,8 +169,9 @@ def attend_block_scaled(
     q_at = q.data_ptr()
     if q_at % 16 or q_tok % 8 or q_head % 8:
         raise _lib.ShiftError("q's rows must start on 16-byte boundaries")
-    if not 0 <= max_query_len < 2**31 or not 0 <= max_seq_len < 2**31 or not 0 <= window < 2**31:
-        raise _lib.ShiftError("max_query_len, max_seq_len and window must be non-negative int32s")
+    if not 0 <= max_query_len < 2**31 or not 0 <= max_seq_len <= 2**30 or not 0 <= window < 2**31:
+        raise _lib.ShiftError("max_query_len and window must be non-negative int32s, max_seq_len at most "
+                              "2^30 and non-negative")
     scale = head_size ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise _lib.ShiftError(f"scale must be finite, got {scale}")

@@ -583,18 +583,23 @@ int attend_dispatch(const AttendArgs& a, int head_size, cudaStream_t stream) {
   return e == cudaSuccess ? MSHIFT_OK : cuda_fail(e);
 }
 
-constexpr int kMaxSplits = 1024;
 // Rows of a request up to which the few-rows kernel is the faster: 64 requests of 32 rows over 8,192 keys take
 // it 514 us and the other 621, of 64 rows 999 and 657; 4 requests of 32 rows 66 and 72, of 64 rows 104 and 76.
 constexpr int kFewRows = 32;
 
-// Tokens of a split, a multiple of 128, between least and most.  Enough splits that the CTAs of
-// all units fill `want` places, but none so short that its start-up shows.
-int chunk_for(int64_t units, int64_t want, int max_len, int64_t least, int64_t most) {
-  const int64_t splits = units > 0 ? (want + units - 1) / units : 1;
-  int64_t chunk = splits <= 1 ? most : ((int64_t)max_len + splits - 1) / splits;
-  chunk = chunk < least ? least : chunk > most ? most : chunk;
-  const int64_t floor = ((int64_t)max_len + kMaxSplits - 1) / kMaxSplits;
+// Keys of a split of the few-rows kernel, a multiple of 128.  Enough splits that the CTAs of all units
+// fill the 148 SMs' four places each; none shorter than 256, whose start-up would show, nor longer than
+// 4,096, so that requests far shorter than the bound still end together; but past what fills the GPU
+// never more than 32, nor than 1 GB of partial results (`bytes` a split) allow, since those go by
+// the bound and not by the lengths.
+int few_chunk(int64_t units, int max_len, int64_t bytes) {
+  const int64_t fill = units > 0 ? (148 * 4 + units - 1) / units : 1;
+  int64_t most = bytes > 0 ? (1ll << 30) / bytes : 32;
+  most = most > 32 ? 32 : most;
+  most = most < fill ? fill : most;
+  int64_t chunk = ((int64_t)max_len + fill - 1) / fill;
+  chunk = chunk < 256 ? 256 : chunk > 4096 ? 4096 : chunk;
+  const int64_t floor = ((int64_t)max_len + most - 1) / most;
   if (chunk < floor) chunk = floor;
   return (int)((chunk + 127) / 128 * 128);
 }
@@ -610,7 +615,8 @@ int rows_chunk(int64_t units, int max_len, int64_t elements) {
   const double part = (double)elements * 8 / 6.5e12 / 2.3e-6;  // of a split, in tiles
   int64_t best = 1;
   double least = 0.0;
-  for (int64_t s = 1; s <= 64 && (s == 1 || tiles / s >= 8); ++s) {
+  // at most 64 splits, of at least 8 tiles, with at most 1 GB of partial results
+  for (int64_t s = 1; s <= 64 && (s == 1 || (tiles / s >= 8 && s * elements * 4 <= 1ll << 30)); ++s) {
     const double rounds = (double)((units * s + 147) / 148);
     const double cost = rounds * ((double)((tiles + s - 1) / s) + 5.0) + (s > 1 ? (double)s * part + 3.0 : 0.0);
     if (s == 1 || cost < least) {
@@ -634,10 +640,11 @@ Plan plan(int32_t rows, int32_t hq, int32_t hk, int32_t head_size, int32_t reqs,
   p.few_rows = head_size > 128 ? INT32_MAX : kFewRows;
   const int64_t few = all < p.few_rows ? all : p.few_rows;
   const int64_t tiles = few <= 8 ? 1 : (few + 15) / 16;
-  p.chunk = chunk_for((int64_t)reqs * hk * tiles, 148 * 4, max_len, 256, 4096);
-  p.nsplit = max_len > 0 ? (int)(((int64_t)max_len + p.chunk - 1) / p.chunk) : 1;
   p.cap = (int64_t)reqs * hk * few <= (int64_t)rows * hq ? few : 0;
-  if (p.nsplit > 1) p.parts = (p.cap ? (int64_t)reqs * hk * p.cap : (int64_t)rows * hq) * p.nsplit;
+  const int64_t partial = p.cap ? (int64_t)reqs * hk * p.cap : (int64_t)rows * hq;
+  p.chunk = few_chunk((int64_t)reqs * hk * tiles, max_len, partial * (head_size + 2) * 4);
+  p.nsplit = max_len > 0 ? (int)(((int64_t)max_len + p.chunk - 1) / p.chunk) : 1;
+  if (p.nsplit > 1) p.parts = partial * p.nsplit;
   p.rchunk = 1 << 30;
   p.rsplit = 1;
   if (all > p.few_rows) {
@@ -653,12 +660,14 @@ Plan plan(int32_t rows, int32_t hq, int32_t hk, int32_t head_size, int32_t reqs,
 }  // namespace serve
 }  // namespace mshift
 
+static constexpr int32_t kMaxSeqLen = 1 << 30;  // key positions and their sums stay within int32
+
 extern "C" {
 
 int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk, int32_t head_size,
                                 int32_t reqs, int32_t max_query_len, int32_t max_seq_len) {
   if (rows < 0 || hq <= 0 || hk <= 0 || hq % hk != 0 || head_size <= 0 || reqs < 0 ||
-      max_query_len < 0 || max_seq_len < 0)
+      max_query_len < 0 || max_seq_len < 0 || max_seq_len > kMaxSeqLen)
     return -1;
   if (rows == 0 || reqs == 0) return 0;
   const auto p = mshift::serve::plan(rows, hq, hk, head_size, reqs, max_query_len, max_seq_len);
@@ -676,7 +685,7 @@ int mshift_attend_block_scaled(
   using namespace mshift;
   using namespace mshift::serve;
   if (paged == nullptr || rows < 0 || reqs < 0 || hq <= 0 || width < 0 || table_stride < width ||
-      max_query_len < 0 || max_seq_len < 0 || window < 0)
+      max_query_len < 0 || max_seq_len < 0 || max_seq_len > kMaxSeqLen || window < 0)
     return MSHIFT_EINVAL;
   if (paged->dtype != MSHIFT_E4M3 || (dtype != MSHIFT_BF16 && dtype != MSHIFT_F16))
     return MSHIFT_EUNSUPPORTED;

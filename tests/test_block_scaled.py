@@ -606,3 +606,16 @@ def test_refusals(cuda):
     ):
         with pytest.raises(ShiftError, match=match):
             append_block_scaled(*args, *c.step, 16, "nhd")
+
+
+def test_workspaces_stay_small_whatever_the_bounds():
+    """Partial results go by the caller's bounds: a loose one must not ask for more than a few GB."""
+    lib = _lib.load()
+    r = random.Random(0)
+    for _ in range(5000):
+        hk, group = r.choice([1, 2, 4, 8]), r.choice([1, 2, 5, 16])
+        args = (r.randint(1, 20000), hk * group, hk, r.choice([64, 128, 256]), r.randint(1, 256),
+                r.choice([1, 4, r.randint(1, 20000)]), r.choice([1, 100, 40000, 1 << 20, 1 << 30]))
+        assert 0 <= lib.mshift_attend_workspace(*args) <= 3 << 30, args
+    assert lib.mshift_attend_workspace(256, 32, 8, 128, 256, 1, 1 << 20) < 200 << 20
+    assert lib.mshift_attend_workspace(1, 4, 2, 64, 1, 1, (1 << 30) + 1) == -1
