@@ -80,7 +80,8 @@ __device__ __forceinline__ int block_column(const AttendArgs& a, int t) {
   return (int)((__umulhi((uint32_t)t, a.bs_mul) + (uint32_t)t) >> a.bs_shift);
 }
 
-// One request's lengths, bounded by what the call's arrays hold.
+// One request's lengths, bounded by what the call's arrays hold.  Rows past the caller's bound have
+// no place in the workspace, which the bound sized: no kernel sees them.
 struct Request {
   int q0, n, seq;
   long long start;  // position of its first row
@@ -89,13 +90,14 @@ struct Request {
 __device__ __forceinline__ Request request_of(const AttendArgs& a, int r, bool report) {
   Request x;
   x.q0 = row_start(a.qs, r, a.rows);
-  x.n = max(row_start(a.qs, r + 1, a.rows) - x.q0, 0);
+  const int n = max(row_start(a.qs, r + 1, a.rows) - x.q0, 0);
+  x.n = min(n, a.max_q);
   const int len = a.lens[r];
-  x.start = (long long)len - x.n;
+  x.start = (long long)len - n;
   const long long held = (long long)a.width * a.bs;
   x.seq = (int)min((long long)min(max(len, 0), a.max_len), held);
   if (report) {
-    if (len > a.max_len || len < 0 || x.n > a.max_q || x.start < 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+    if (len > a.max_len || len < 0 || n > a.max_q || x.start < 0) flag(a.err, MSHIFT_ERR_LENGTHS);
     if (len > held) flag(a.err, MSHIFT_ERR_POOL);
   }
   return x;

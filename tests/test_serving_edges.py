@@ -1,0 +1,107 @@
+"""Edges of the serving operators: bounds that a request passes, NaN, flagged lengths, what is refused."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import serving
+from marathon_b200 import _lib
+from marathon_b200._serve import geometry
+from marathon_b200.block_scaled import attend_block_scaled
+from marathon_b200.shift_kernels import take_errors
+from test_block_scaled import Case, _cum, _i32
+
+
+def _attend(c, **kw):
+    """The call without ``check``, so that what it flags is left for the test."""
+    return attend_block_scaled(*c.dev, *c.step, c.bs, c.layout, return_lse=True, **{**c.bounds, **kw})
+
+
+def _check_rows(c, got, rows, **kw):
+    """The listed rows against the formula, within the tolerances of test_block_scaled.py."""
+    out, lse = (x.cpu().double()[rows] for x in got)
+    want, wlse, mag, big = (x[rows] for x in serving.attend(
+        c.q, c.kv, c.ks, c.vs, c.tables, c.qs, c.lens, c.bs, c.layout, c.d**-0.5, **kw))
+    d = 2.0**-20 * big
+    tol = torch.finfo(c.q.dtype).eps / 2 * want.abs() + (2.0**-11 + 2.0**-20 + d[..., None]) * mag
+    assert bool(((out - want).abs() <= tol).all())
+    none = wlse == -math.inf
+    assert torch.equal(none, lse == -math.inf) and bool((out[none] == 0).all())
+    off = torch.where(none, 0.0, (lse - wlse).abs())
+    assert bool((off <= d + 2.0**-20 + 2.0**-22 * torch.where(none, 0.0, wlse).abs()).all())
+
+
+# ------------------------------------------------------ rows past max_query_len
+PAST = [  # rows of the requests, bound, query heads, KV heads, head size: few rows, several tiles, many rows
+    ([1, 2, 1, 3], 1, 10, 2, 128),
+    ([2, 1, 9], 1, 4, 4, 64),
+    ([2, 9, 1], 2, 8, 2, 256),
+    ([7, 3, 40], 3, 10, 2, 128),
+    ([90, 30, 200], 60, 4, 2, 64),
+]
+
+
+def _past(cuda, new, hq, hk, d):
+    lens = [700 + 311 * i + n for i, n in enumerate(new)]
+    return Case(cuda, lens, new, hq, hk, d, 16, seed=len(new) + d, pad=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [2000, 30720])
+@pytest.mark.parametrize("new,bound,hq,hk,d", PAST)
+def test_rows_past_the_query_bound_are_left_and_the_others_right(cuda, new, bound, hq, hk, d, most):
+    """One request or more has more rows than the caller's bound, with splits of the keys."""
+    take_errors(cuda)
+    c = _past(cuda, new, hq, hk, d)
+    out = torch.full((c.q.shape[0], hq, d), 7.0, dtype=c.q.dtype, device=cuda)
+    got = _attend(c, max_query_len=bound, max_seq_len=most, out=out)
+    assert take_errors(cuda) == _lib.ERR_LENGTHS
+    rows = [q + i for q, n in zip(c.qs, new, strict=False) for i in range(min(n, bound))]
+    _check_rows(c, got, rows)
+    rest = [i for i in range(c.q.shape[0]) if i not in set(rows)]
+    assert bool((out[rest] == 7).all()) and bool((got[1][rest] == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,bound,hq,hk,d", PAST)
+def test_rows_past_the_query_bound_leave_what_is_behind_the_workspace(cuda, new, bound, hq, hk, d):
+    take_errors(cuda)
+    c = _past(cuda, new, hq, hk, d)
+    lib, rows, most = _lib.load(), c.q.shape[0], 30720
+    geo, paged = geometry(c.dev[1], c.bs, c.layout)
+    need = lib.mshift_attend_workspace(rows, hq, hk, d, len(new), bound, most)
+    assert need > 0
+    work = torch.full((need + (1 << 20),), 0x5A, dtype=torch.uint8, device=cuda)
+    out = torch.zeros_like(c.dev[0])
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    kv, ks, vs = c.dev[1:]
+    tables, qs, lens = c.step
+    status = lib.mshift_attend_block_scaled(
+        _lib.BF16, c.dev[0].data_ptr(), hq * d, d, rows, hq, paged, kv.data_ptr(),
+        kv.data_ptr() + geo.v_offset, ks.data_ptr(), *ks.stride(), vs.data_ptr(), *vs.stride(),
+        tables.data_ptr(), tables.stride(0), tables.shape[1], qs.data_ptr(), lens.data_ptr(), len(new),
+        bound, most, d**-0.5, 1, 0, out.data_ptr(), hq * d, d, None, 0, work.data_ptr(), need,
+        err.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert status == _lib.OK
+    assert int(err.item()) == _lib.ERR_LENGTHS
+    assert bool((work[need:] == 0x5A).all())
+
+
+@pytest.mark.gpu
+def test_a_graph_captured_for_one_token_and_replayed_with_two(cuda):
+    """The bound a graph was captured with is passed by its replay's lengths: flagged, the others right."""
+    c = _past(cuda, [1, 1, 1], 8, 2, 128)
+    want = c.run(max_query_len=1, max_seq_len=30720)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = _attend(c, max_query_len=1, max_seq_len=30720)
+    g.replay()
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and take_errors(cuda) == 0
+    c.step[1].copy_(_i32(cuda, _cum([2, 1, 1])))  # one of the rows of padding becomes a token
+    c.new, c.qs = [2, 1, 1], _cum([2, 1, 1])
+    g.replay()
+    assert take_errors(cuda) == _lib.ERR_LENGTHS
+    _check_rows(c, (out, lse), [0, 2, 3])
