@@ -348,11 +348,11 @@ MSHIFT_API int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk,
  * j / (hq / heads)) over the cache: row at position x sees the keys [0, x] of its request
  * (all of them without `causal`), and of those the last `window` if window > 0.
  * out [rows, hq, head_size] of q's dtype; lse [rows, hq] fp32 (natural log) or NULL.
- * A row that sees no key gets zeros and -inf.  Rows of no request are left as they were,
- * or zeroed if zero_tail.  max_query_len / max_seq_len bound the requests' rows and
- * lengths (max_seq_len at most 2^30); a request past them is cut off there and sets
- * MSHIFT_ERR_LENGTHS.  Keys in
- * a bad block count as unseen.  Value scales are positive; below 2^-64 they are read as 2^-64.
+ * A row that sees no key gets zeros and -inf.  max_query_len / max_seq_len bound the requests'
+ * rows and lengths (max_seq_len at most 2^30); a request past them is cut off there and sets
+ * MSHIFT_ERR_LENGTHS.  Rows of no request and rows past max_query_len are left as they were, or
+ * get zeros and -inf if zero_tail.  Keys in a bad block count as unseen.  Value scales are
+ * positive; below 2^-64 they are read as 2^-64.
  * q, out, the cache and workspace start on 16-byte boundaries, as do their rows.
  */
 MSHIFT_API int mshift_attend_block_scaled(int32_t dtype, const void* q, int64_t q_tok,

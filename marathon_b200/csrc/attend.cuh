@@ -84,6 +84,7 @@ __device__ __forceinline__ int block_column(const AttendArgs& a, int t) {
 // no place in the workspace, which the bound sized: no kernel sees them.
 struct Request {
   int q0, n, seq;
+  int past;         // rows left out behind its n
   long long start;  // position of its first row
 };
 
@@ -92,6 +93,7 @@ __device__ __forceinline__ Request request_of(const AttendArgs& a, int r, bool r
   x.q0 = row_start(a.qs, r, a.rows);
   const int n = max(row_start(a.qs, r + 1, a.rows) - x.q0, 0);
   x.n = min(n, a.max_q);
+  x.past = n - x.n;
   const int len = a.lens[r];
   x.start = (long long)len - n;
   const long long held = (long long)a.width * a.bs;

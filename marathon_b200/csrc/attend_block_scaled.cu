@@ -93,16 +93,18 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
+  // with zero_tail the result is new memory: rows that nothing else writes become zeros
+  auto clear = [&](int64_t row, int head, int heads) {
+    for (int i = threadIdx.x; i < heads * D; i += kWarps * 32)
+      static_cast<T*>(a.out)[row * a.o_tok + (head + i / D) * a.o_head + i % D] = Elem<T>::put(0.0f);
+    for (int i = threadIdx.x; i < heads && a.lse != nullptr; i += kWarps * 32)
+      a.lse[row * a.hq + head + i] = -INFINITY;
+  };
   if (a.zero_tail) {  // rows of no request
     const int before = row_start(a.qs, 0, a.rows), behind = row_start(a.qs, a.reqs, a.rows);
     const int64_t none = before + (int64_t)a.rows - behind;
-    for (int64_t i0 = blockIdx.x; i0 < none; i0 += gridDim.x) {
-      const int64_t row = i0 < before ? i0 : i0 - before + behind;
-      for (int i = threadIdx.x; i < a.hq * D; i += kWarps * 32)
-        static_cast<T*>(a.out)[row * a.o_tok + (i / D) * a.o_head + i % D] = Elem<T>::put(0.0f);
-      for (int i = threadIdx.x; i < a.hq && a.lse != nullptr; i += kWarps * 32)
-        a.lse[row * a.hq + i] = -INFINITY;
-    }
+    for (int64_t i = blockIdx.x; i < none; i += gridDim.x)
+      clear(i < before ? i : i - before + behind, 0, a.hq);
   }
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be made ready
   // heads fastest: in the NHD layouts neighbouring CTAs read neighbouring bytes
@@ -114,6 +116,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
   const int split = (int)(id % a.nsplit);
   const int r = (int)(id / a.nsplit);
   const Request rq = request_of(a, r, threadIdx.x == 0 && h == 0 && tile == 0 && split == 0);
+  if (a.zero_tail && tile == 0 && split == 0)  // rows past the caller's bound
+    for (int i = 0; i < rq.past; ++i) clear(rq.q0 + rq.n + i, h * a.group, a.group);
   const int all = rq.n * a.group, m0 = tile * kRows;
   if (all > a.few_rows || m0 >= all) return;
   const int live = min(kRows, all - m0);

@@ -105,3 +105,20 @@ def test_a_graph_captured_for_one_token_and_replayed_with_two(cuda):
     g.replay()
     assert take_errors(cuda) == _lib.ERR_LENGTHS
     _check_rows(c, (out, lse), [0, 2, 3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [2000, 30720])
+@pytest.mark.parametrize("new,bound,hq,hk,d", PAST)
+def test_rows_past_the_query_bound_are_zeros_in_a_new_result(cuda, new, bound, hq, hk, d, most):
+    take_errors(cuda)
+    c = _past(cuda, new, hq, hk, d)
+    junk = [torch.full((c.q.shape[0], hq, w), 7.0, dtype=t, device=cuda)
+            for w, t in ((d, c.q.dtype), (1, torch.float32))]
+    del junk  # what a result's memory may hold before
+    out, lse = _attend(c, max_query_len=bound, max_seq_len=most)
+    assert take_errors(cuda) == _lib.ERR_LENGTHS
+    rows = [q + i for q, n in zip(c.qs, new, strict=False) for i in range(min(n, bound))]
+    _check_rows(c, (out, lse), rows)
+    rest = [i for i in range(c.q.shape[0]) if i not in set(rows)]
+    assert bool((out[rest] == 0).all()) and bool((lse[rest] == -math.inf).all())
