@@ -113,5 +113,9 @@ __device__ __forceinline__ int2 seen(const AttendArgs& a, const Request& rq, lon
   return make_int2((int)lo, (int)hi);
 }
 
+// Whether a row with this M and l has seen a key.  No comparison passes for NaN, so a row whose scores
+// all are leaves M where it was, but its l is NaN then: it gets NaN, not the zeros of a row without keys.
+__device__ __forceinline__ bool has_key(float M, float l) { return M > kNoKey || l != l; }
+
 }  // namespace serve
 }  // namespace mshift

@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
       *reinterpret_cast<float4*>(a.part_o + part * D + d) = make_float4(x[0], x[1], x[2], x[3]);
       if (d == 0) a.part_ml[part] = make_float2(top, sum);
     } else {
-      const bool any = top > kNoKey;
+      const bool any = has_key(top, sum);
       const float by = any ? 1.0f / sum : 0.0f;
       T* dst = static_cast<T*>(a.out) + row * a.o_tok + hq * a.o_head + d;
 #pragma unroll
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
       for (int e = 0; e < kVec; ++e) x[e] += s_x[warp + w][lane * kVec + e];
   }
-  const bool any = top > kNoKey;
+  const bool any = has_key(top, sum);
   T* dst = static_cast<T*>(a.out) + row * a.o_tok + hq * a.o_head + lane * kVec;
 #pragma unroll
   for (int e = 0; e < kVec; ++e) x[e] = any ? x[e] / sum : 0.0f;

@@ -469,10 +469,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return Elem<T>::pack(f);
 }
 
+// Whether one of the keys lies in a block of the cache.  Only rows of NaN ask.
+__device__ __forceinline__ bool any_block(const AttendArgs& a, int r, int2 see) {
+  bool any = false;
+#pragma unroll 1
+  for (int key = see.x; !any && key < see.y; key = (block_column(a, key) + 1) * a.bs) {
+    const int b = a.tables[(int64_t)r * a.tab_stride + block_column(a, key)];
+    any = b >= 0 && b < a.num_blocks;
+  }
+  return any;
+}
+
 // Rows 32 * (warp % 4) + lane of tile t.
 template <int D, bool PAGE16, typename T>
-__device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const Request& rq, int h,
-                                        int m0, int split, const Span sp, int all) {
+__device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const Request& rq, int r,
+                                        int h, int m0, int split, const Span sp, int all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = warp >> 2, row = (warp & 3) * 32 + lane;
   const int m = m0 + t * kTile + row;
@@ -662,7 +673,9 @@ __device__ __forceinline__ void softmax(const AttendArgs& a, Smem<D>& s, const R
   if (ok) ok = __all_sync(0xffffffffu, bar_wait(&s.done, 0, &s.gone, a.err));
   if (!ok || s.gone) return;
   fence_after();
-  const bool any = M > kNoKey;
+  // keys in bad blocks are unseen by a row of NaN too, whose product with their zeros is NaN
+  if (M == kNoKey && l != l && !any_block(a, r, see)) l = 0.0f;
+  const bool any = has_key(M, l);
   const float by = any ? 1.0f / l : 0.0f;
   const int64_t part = (tok * a.hq + hq) * a.rsplit + split;
   if (live && a.rsplit > 1)
@@ -812,7 +825,7 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
   // 256 * 176 + 128 * 112 + 128 * 48 = 512 * 128 registers
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    softmax<D, PAGE16, T>(a, s, rq, h, m0, split, sp, all);
+    softmax<D, PAGE16, T>(a, s, rq, r, h, m0, split, sp, all);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     loader<D>(a, s, h, sp.tiles);

@@ -12,7 +12,7 @@ from marathon_b200 import _lib
 from marathon_b200._serve import geometry
 from marathon_b200.block_scaled import attend_block_scaled
 from marathon_b200.shift_kernels import take_errors
-from test_block_scaled import Case, _cum, _i32
+from test_block_scaled import NAN_CODE, Case, _cum, _i32
 
 
 def _attend(c, **kw):
@@ -122,3 +122,49 @@ def test_rows_past_the_query_bound_are_zeros_in_a_new_result(cuda, new, bound, h
     _check_rows(c, (out, lse), rows)
     rest = [i for i in range(c.q.shape[0]) if i not in set(rows)]
     assert bool((out[rest] == 0).all()) and bool((lse[rest] == -math.inf).all())
+
+
+# ------------------------------------------------------------------------ NaN
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [700, 40000])
+@pytest.mark.parametrize("new,d,bs", [(1, 128, 16), (2, 64, 24), (60, 128, 16), (60, 64, 24), (40, 256, 16)])
+def test_nan_queries_give_nan_and_no_empty_rows(cuda, new, d, bs, most):
+    c = Case(cuda, [700, 90], [new, new], 4, 2, d, bs, seed=3)
+    good = c.run(max_seq_len=most)
+    for at, head in ((0, 1), (new - 1, 2), (new, 3), (2 * new - 1, 0)):
+        was = c.dev[0]
+        c.dev[0] = was.clone()
+        c.dev[0][at, head, 5] = float("nan")
+        out, lse = c.run(max_seq_len=most)
+        c.dev[0] = was
+        hit = torch.zeros(2 * new, 4, dtype=torch.bool, device=cuda)
+        hit[at, head] = True
+        assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
+        assert torch.equal(out[~hit], good[0][~hit]) and torch.equal(lse[~hit], good[1][~hit])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [60, 40000])
+@pytest.mark.parametrize("new,d", [(1, 128), (60, 128), (60, 64), (7, 256)])
+def test_rows_whose_only_keys_are_nan(cuda, new, d, most):
+    take_errors(cuda)
+    c = Case(cuda, [new, 5], [new, 5], 4, 2, d, 16, seed=4)
+    good = c.run(max_seq_len=most)
+    c.dev[1] = c.dev[1].clone()
+    serving.sides(c.dev[1].view(torch.uint8), "nhd")[0][c.tables[0][0], 0, 1, 7] = NAN_CODE  # the first key, KV head 1
+    out, lse = c.run(max_seq_len=most)
+    assert bool(out[:new, 2:].isnan().all()) and bool(lse[:new, 2:].isnan().all())
+    assert torch.equal(out[:, :2], good[0][:, :2]) and torch.equal(lse[:, :2], good[1][:, :2])
+    assert torch.equal(out[new:], good[0][new:])
+    c = Case(cuda, [9, 5], [9, 1], 4, 2, d, 16, seed=4)
+    c.dev[2] = c.dev[2].clone()
+    c.dev[2][c.tables[0][0], 0] = float("nan")
+    out, lse = c.run(max_seq_len=most)
+    assert bool(out[:9, :2].isnan().all()) and bool(lse[:9, :2].isnan().all())
+    assert bool(out[:9, 2:].isfinite().all()) and bool(out[9:].isfinite().all())
+    # keys in bad blocks count as unseen, to a row of NaN too
+    c.dev[0] = torch.full_like(c.dev[0], float("nan"))
+    c.step[0] = torch.full_like(c.step[0], -1)
+    out, lse = _attend(c, max_seq_len=most)
+    assert take_errors(cuda) == _lib.EBIT_SLOT
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
