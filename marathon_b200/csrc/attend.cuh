@@ -23,7 +23,7 @@ namespace mshift {
 namespace serve {
 
 constexpr float kLazy = 8.0f;            // log2 of how far P may pass 1 before a rescale
-constexpr float kNoKey = -1e30f;         // M of a row that has seen no key
+constexpr float kNoKey = -3.402823466e38f;  // M of a row that has seen no key: below every score
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -168,3 +168,23 @@ def test_rows_whose_only_keys_are_nan(cuda, new, d, most):
     out, lse = _attend(c, max_seq_len=most)
     assert take_errors(cuda) == _lib.EBIT_SLOT
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [64, 40000])
+@pytest.mark.parametrize("new,d", [(1, 128), (40, 128), (40, 64), (4, 256)])
+def test_scores_far_below_zero_are_scores(cuda, new, d, most):
+    c = Case(cuda, [40], [new], 4, 2, d, 16, seed=5, pow2=True)
+    k, v = serving.sides(c.kv.view(torch.uint8), "nhd")
+    for p in range(40):  # key p's codes are all alike, larger for later keys
+        k[c.tables[0][p // 16], p % 16] = 8 + p
+    c.q = torch.full_like(c.q, -(2.0**110))
+    c.ks = torch.ones_like(c.ks)
+    c.dev = [x.to(cuda) for x in (c.q, c.kv, c.ks, c.vs)]
+    out, lse = c.run(max_seq_len=most)
+    # the first key's score is 2^100 above the next one's: all the weight
+    first = v[c.tables[0][0], 0].view(torch.float8_e4m3fn).double() * c.vs[c.tables[0][0]].double()[:, None]
+    want = first.repeat_interleave(2, 0).expand(new, 4, d)
+    assert bool(((out.cpu().double() - want).abs() <= 2.0**-8 * want.abs()).all())
+    score = -(2.0**110) * d * 2.0**-6 * d**-0.5
+    assert bool(((lse.cpu().double() / score - 1).abs() <= 2.0**-20).all())
