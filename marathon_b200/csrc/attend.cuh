@@ -113,6 +113,17 @@ __device__ __forceinline__ int2 seen(const AttendArgs& a, const Request& rq, lon
   return make_int2((int)lo, (int)hi);
 }
 
+// The keys [lo, hi) that some of a tile's rows see, those at positions first to last: later rows see later
+// keys at both ends.  The last row's window may be empty where an earlier row's is not, behind a length
+// that was cut.
+__device__ __forceinline__ int2 seen_by_tile(const AttendArgs& a, const Request& rq, long long first,
+                                             long long last) {
+  const long long hi = a.causal ? min(last + 1, (long long)rq.seq) : rq.seq;
+  const long long lo = a.window > 0 ? max(max(first, 0ll) - a.window + 1, 0ll) : 0;
+  if (last < 0 || hi <= lo) return make_int2(0, 0);
+  return make_int2((int)lo, (int)hi);
+}
+
 // Whether a row with this M and l has seen a key.  No comparison passes for NaN, so a row whose scores
 // all are leaves M where it was, but its l is NaN then: it gets NaN, not the zeros of a row without keys.
 __device__ __forceinline__ bool has_key(float M, float l) { return M > kNoKey || l != l; }

@@ -131,14 +131,14 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
       const int m = i * 8 + 2 * c + e;
       mine[i][e] = m < live ? seen(a, rq, rq.start + (m0 + m) / a.group) : make_int2(0, 0);
     }
-  const int2 head = seen(a, rq, max(rq.start + m0 / a.group, 0ll));
-  const int2 last = seen(a, rq, rq.start + (m0 + live - 1) / a.group);
-  // rows later in the tile see later keys at both ends
-  const int lo = max(head.x, split * a.chunk);
-  const int hi = min(last.y, split * a.chunk + a.chunk);
-  const int full_lo = max(last.x, lo);                       // keys that every row sees
-  const int full_hi = min(a.causal ? head.y : last.y, hi);
-  const bool all_live = rq.start + m0 / a.group >= 0;
+  const long long first_at = rq.start + m0 / a.group, last_at = rq.start + (m0 + live - 1) / a.group;
+  const int2 tile_see = seen_by_tile(a, rq, first_at, last_at);
+  const int2 head = seen(a, rq, max(first_at, 0ll)), last = seen(a, rq, last_at);
+  const int lo = max(tile_see.x, split * a.chunk);
+  const int hi = min(tile_see.y, split * a.chunk + a.chunk);
+  const int full_lo = max(last.x, lo);  // keys that every row sees
+  const int full_hi = min(a.causal ? min(head.y, last.y) : last.y, hi);
+  const bool all_live = first_at >= 0;
 
   const int32_t* table = a.tables + (int64_t)r * a.tab_stride;
   const uint8_t* kh = a.k + h * a.head;

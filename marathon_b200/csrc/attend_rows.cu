@@ -778,10 +778,9 @@ __global__ void __launch_bounds__(kCta, 1) attend_rows_kernel(const AttendArgs a
   const int last_m = min(m0 + 2 * kTile, all) - 1;
   Span sp;
   {
-    const int2 head = seen(a, rq, max(rq.start + m0 / a.group, 0ll));
-    const int2 last = seen(a, rq, rq.start + last_m / a.group);
-    sp.lo = max(head.x, split * a.rchunk);
-    sp.hi = (int)min((long long)last.y, (long long)split * a.rchunk + a.rchunk);
+    const int2 see = seen_by_tile(a, rq, rq.start + m0 / a.group, rq.start + last_m / a.group);
+    sp.lo = max(see.x, split * a.rchunk);
+    sp.hi = (int)min((long long)see.y, (long long)split * a.rchunk + a.rchunk);
     sp.first = sp.lo / kTile * kTile;
     sp.tiles = sp.hi > sp.lo ? (sp.hi - sp.first + kTile - 1) / kTile : 0;
   }

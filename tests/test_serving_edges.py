@@ -188,3 +188,47 @@ def test_scores_far_below_zero_are_scores(cuda, new, d, most):
     assert bool(((out.cpu().double() - want).abs() <= 2.0**-8 * want.abs()).all())
     score = -(2.0**110) * d * 2.0**-6 * d**-0.5
     assert bool(((lse.cpu().double() / score - 1).abs() <= 2.0**-20).all())
+
+
+# ------------------------------------------------------- windows and cut lengths
+def _formula(c, at, key_end, window, group):
+    """Rows at positions `at` of request 0: keys below key_end, causal, windowed."""
+    kc, vc = serving.sides(c.kv, c.layout)
+    ids = torch.tensor(c.tables[0][: -(-key_end // c.bs)])
+    kk = (kc[ids].double() * c.ks[ids].double()[:, None, :, None]).reshape(-1, c.hk, c.d)
+    vv = (vc[ids].double() * c.vs[ids].double()[:, None, :, None]).reshape(-1, c.hk, c.d)
+    out = torch.zeros(len(at), c.q.shape[1], c.d, dtype=torch.float64)
+    lse = torch.full(out.shape[:2], -math.inf, dtype=torch.float64)
+    for i, x in enumerate(at):
+        lo, hi = max(x - window + 1, 0), min(x + 1, key_end)
+        for h in range(c.q.shape[1]) if lo < hi else ():
+            s = kk[lo:hi, h // group] @ c.q[i, h].double() * c.d**-0.5
+            lse[i, h] = torch.logsumexp(s, 0)
+            out[i, h] = torch.softmax(s, 0) @ vv[lo:hi, h // group]
+    return out, lse
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 128), (8, 2, 128), (8, 2, 64), (2, 1, 256)])
+@pytest.mark.parametrize("cut", ["bound", "table"])
+@pytest.mark.parametrize("long", [0, 5120])
+def test_windows_of_requests_cut_at_a_bound(cuda, hq, hk, d, cut, long):
+    """Rows behind a cut length whose window still reaches a key see it, the others nothing; with and
+    without splits."""
+    take_errors(cuda)
+    c = Case(cuda, [long + 100], [20], hq, hk, d, 16, seed=6)
+    if cut == "bound":
+        got, flag, end = _attend(c, max_seq_len=long + 90, window=5), _lib.ERR_LENGTHS, long + 90
+    else:
+        c.step[0] = c.step[0][:, : (long + 80) // 16]
+        got, flag, end = _attend(c, max_seq_len=2 * long + 100, window=5), _lib.ERR_POOL, long + 80
+    assert take_errors(cuda) == flag
+    want, wlse = _formula(c, range(long + 80, long + 100), end, 5, hq // hk)
+    out, lse = (x.cpu().double() for x in got)
+    none = wlse == -math.inf
+    assert torch.equal(none, lse == -math.inf) and bool((out[none] == 0).all())
+    # the tolerances of test_block_scaled.py with what bounds their terms here: |o| <= A <= 448 * 0.023 and
+    # sum |q||k| scale < 2^8 * 448 * 0.023 * 5 / 8 < 2^11
+    assert bool((torch.where(none, 0.0, lse - wlse).abs() <= 2.0**-9).all())
+    assert bool(((out - want).abs() <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-20 + 2.0**-9) * 10.4).all())
+    assert not bool(none[:4].any()) and bool(none[-4:].all())
