@@ -298,7 +298,8 @@ MSHIFT_API int mshift_enable_peer(int32_t peer_device);
  * `tokens` rows slots (block * block_size + offset) and positions; rows behind the
  * last request get slot -1, position 0.  free_head_out (not free_head itself) gets the
  * new head.  Too few free blocks, or a table too narrow: slot -1 and MSHIFT_ERR_POOL.
- * More new tokens than `tokens`: the surplus is dropped and MSHIFT_ERR_LENGTHS set.
+ * More new tokens than `tokens`: the surplus is dropped, takes no blocks, and MSHIFT_ERR_LENGTHS
+ * is set.
  */
 MSHIFT_API int mshift_block_maps(const int32_t* cached_lens, const int32_t* new_lens,
                 int32_t reqs, int32_t* block_tables, int64_t table_stride, int32_t width,

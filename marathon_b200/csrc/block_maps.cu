@@ -54,10 +54,12 @@ __global__ void __launch_bounds__(kMapThreads) block_maps_kernel(const MapArgs a
   __shared__ long long s_start[kMapThreads], s_end[kMapThreads], s_block[kMapThreads];
   __shared__ long long s_warp[2][32];
   __shared__ int s_scan[32];
+  __shared__ long long s_used;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long t0 = (long long)blockIdx.x * kMapThreads;
   const int head = *a.free_head;
   s_req[tid] = -1;
+  if (tid == 0) s_used = 0;
   __syncthreads();
 
   // 64-bit sums: lengths come from the device and are not trusted to be small
@@ -92,6 +94,9 @@ __global__ void __launch_bounds__(kMapThreads) block_maps_kernel(const MapArgs a
         const long long q1 = min(tok0 + fresh, (long long)a.tokens);
         a.query_start[r] = (int)q0;
         a.seq_lens[r] = (int)min(cached + q1 - q0, (long long)INT32_MAX);
+        // the request in which the bound falls: what is dropped takes no blocks
+        if (tok0 < a.tokens && tok0 + fresh >= a.tokens)
+          s_used = blk0 + (cached + q1 - q0 + a.bs - 1) / a.bs - ((long long)cached + a.bs - 1) / a.bs;
       }
       // requests tile the token axis, so at most one of them starts at, or
       // reaches into the tile at, each place
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(kMapThreads) block_maps_kernel(const MapArgs a
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.query_start[a.reqs] = (int)min(tok_base, (long long)a.tokens);
-    const long long end = (long long)head + blk_base;
+    const long long end = (long long)head + (tok_base > a.tokens ? s_used : blk_base);
     a.free_head_out[0] = (int)min(max(end, 0ll), (long long)a.free_len);
     if (tok_base > a.tokens) flag(a.err, MSHIFT_ERR_LENGTHS);
     if (head < 0 || end > a.free_len) flag(a.err, MSHIFT_ERR_POOL);

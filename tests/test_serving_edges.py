@@ -10,6 +10,7 @@ import torch
 import serving
 from marathon_b200 import _lib
 from marathon_b200._serve import geometry
+from marathon_b200.block_maps import block_maps
 from marathon_b200.block_scaled import attend_block_scaled
 from marathon_b200.shift_kernels import take_errors
 from test_block_scaled import NAN_CODE, Case, _cum, _i32
@@ -232,3 +233,23 @@ def test_windows_of_requests_cut_at_a_bound(cuda, hq, hk, d, cut, long):
     assert bool((torch.where(none, 0.0, lse - wlse).abs() <= 2.0**-9).all())
     assert bool(((out - want).abs() <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-20 + 2.0**-9) * 10.4).all())
     assert not bool(none[:4].any()) and bool(none[-4:].all())
+
+
+# ----------------------------------------------------------------- block maps
+@pytest.mark.gpu
+def test_dropped_tokens_take_no_blocks(cuda):
+    take_errors(cuda)
+    c, n, f, h = (_i32(cuda, x) for x in ([0, 0, 3], [20, 20, 40], [1, 2, 3, 4, 5, 6, 7, 8], [1]))
+    for tokens, head, lens in ((25, 4, [20, 5, 3]), (20, 3, [20, 0, 3]), (0, 1, [0, 0, 3]), (37, 5, [20, 17, 3]),
+                               (45, 5, [20, 20, 8]), (79, 7, [20, 20, 42])):
+        t = torch.full((3, 4), -1, dtype=torch.int32, device=cuda)
+        t[2, 0] = 99
+        got = block_maps(c, n, t, f, h, 16, tokens)
+        assert take_errors(cuda) == _lib.ERR_LENGTHS
+        assert got.seq_lens.tolist() == lens and got.free_head.tolist() == [head], tokens
+        named = [b for row in t.tolist() for b in row if b >= 0 and b != 99]
+        assert named == list(range(2, head + 1)), tokens
+    # too few free blocks for the lengths, enough for the rows
+    t = torch.full((3, 4), -1, dtype=torch.int32, device=cuda)
+    got = block_maps(c, n, t, f[:4], h, 16, 25)
+    assert take_errors(cuda) == _lib.ERR_LENGTHS and got.free_head.tolist() == [4]
