@@ -147,7 +147,10 @@ __global__ void __launch_bounds__(kMapThreads) block_maps_kernel(const MapArgs a
   int block = -1;
   if (col >= have) {
     const long long f = head + s_block[src] + (col - have);
-    if (head >= 0 && f < a.free_len) block = a.free_blocks[f];
+    if (head >= 0 && f < a.free_len) {
+      block = a.free_blocks[f];
+      if (block < 0) flag(a.err, MSHIFT_EBIT_SLOT);
+    }
     if (off == 0 && col < a.width) row[col] = block;
   } else if (col < a.width) {
     block = row[col];

@@ -253,3 +253,13 @@ def test_dropped_tokens_take_no_blocks(cuda):
     t = torch.full((3, 4), -1, dtype=torch.int32, device=cuda)
     got = block_maps(c, n, t, f[:4], h, 16, 25)
     assert take_errors(cuda) == _lib.ERR_LENGTHS and got.free_head.tolist() == [4]
+
+
+@pytest.mark.gpu
+def test_a_free_block_below_zero_is_flagged(cuda):
+    take_errors(cuda)
+    c, n, f, h = (_i32(cuda, x) for x in ([0], [20], [4, -1], [0]))
+    t = torch.full((1, 2), -1, dtype=torch.int32, device=cuda)
+    got = block_maps(c, n, t, f, h, 16, 20)
+    assert take_errors(cuda) == _lib.EBIT_SLOT
+    assert got.slots.tolist() == [64 + i for i in range(16)] + [-1] * 4
