@@ -55,8 +55,9 @@ def block_maps(
 
     Flagged, with slot -1 (``check=True`` synchronises and raises, otherwise
     :func:`~marathon_b200.shift_kernels.take_errors` tells): a free list that runs out, a table too
-    narrow, an old entry or a free block below 0, negative lengths (read as 0), more tokens than
-    ``tokens`` (the surplus is dropped, from ``seq_lens`` too, and takes no blocks).
+    narrow, an old entry or a free block below 0, negative lengths (read as 0), whole lengths
+    past int32 (cut there), more tokens than ``tokens`` (the surplus is dropped, from ``seq_lens`` too,
+    and takes no blocks).
     """
     dev = cuda_on("cached_lens new_lens block_tables free_blocks free_head", cached_lens, new_lens,
                   block_tables, free_blocks, free_head)

@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(kMapThreads) block_maps_kernel(const MapArgs a
     if (r < a.reqs) {
       cached = a.cached[r];
       fresh = a.fresh[r];
-      if ((cached < 0 || fresh < 0) && blockIdx.x == 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+      if ((cached < 0 || fresh < 0 || (long long)cached + fresh > INT32_MAX) && blockIdx.x == 0)
+        flag(a.err, MSHIFT_ERR_LENGTHS);
       cached = max(cached, 0);
       fresh = max(fresh, 0);
     }

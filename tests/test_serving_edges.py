@@ -263,3 +263,13 @@ def test_a_free_block_below_zero_is_flagged(cuda):
     got = block_maps(c, n, t, f, h, 16, 20)
     assert take_errors(cuda) == _lib.EBIT_SLOT
     assert got.slots.tolist() == [64 + i for i in range(16)] + [-1] * 4
+
+
+@pytest.mark.gpu
+def test_lengths_past_32_bits_are_flagged(cuda):
+    take_errors(cuda)
+    c, n, f, h = (_i32(cuda, x) for x in ([2**31 - 2, 5], [4, 1], [0, 1, 2], [0]))
+    t = torch.zeros((2, 2), dtype=torch.int32, device=cuda)
+    got = block_maps(c, n, t, f, h, 2**30, 5)
+    assert take_errors(cuda) & _lib.ERR_LENGTHS
+    assert got.seq_lens.tolist() == [2**31 - 1, 6]
