@@ -181,13 +181,14 @@ def _(q, k, positions, inv_freq, axes=None, inverse=False):
 
 
 def _rotary_axes_setup(ctx, inputs, output) -> None:
-    _, _, *ctx.tables, ctx.inverse = inputs
+    _, _, *tables, ctx.inverse = inputs
+    ctx.save_for_backward(*tables)  # a table changed before the backward pass is noticed there
 
 
 def _rotary_axes_backward(ctx, dq, dk):
     # a sum's gradient comes as one element read many times: the kernel wants contiguous heads
     dq, dk = (d if d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
-    return *torch.ops.marathon.rotary_axes(dq, dk, *ctx.tables, not ctx.inverse), None, None, None, None
+    return *torch.ops.marathon.rotary_axes(dq, dk, *ctx.saved_tensors, not ctx.inverse), None, None, None, None
 
 
 _rotary_axes_op.register_autograd(_rotary_axes_backward, setup_context=_rotary_axes_setup)

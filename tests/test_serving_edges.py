@@ -7,12 +7,14 @@ import math
 import pytest
 import torch
 
+import marathon_b200  # noqa: F401  (registers the operators)
 import serving
 from marathon_b200 import _lib
 from marathon_b200._serve import geometry
 from marathon_b200.block_maps import block_maps
 from marathon_b200.block_scaled import attend_block_scaled
-from marathon_b200.shift_kernels import take_errors
+from marathon_b200.rotary import axis_map, rotary_axes
+from marathon_b200.shift_kernels import inv_freq, take_errors
 from test_block_scaled import NAN_CODE, Case, _cum, _i32
 
 
@@ -273,3 +275,21 @@ def test_lengths_past_32_bits_are_flagged(cuda):
     got = block_maps(c, n, t, f, h, 2**30, 5)
     assert take_errors(cuda) & _lib.ERR_LENGTHS
     assert got.seq_lens.tolist() == [2**31 - 1, 6]
+
+
+# -------------------------------------------------------------------- rotary
+@pytest.mark.gpu
+def test_changed_positions_stop_a_rotary_backward(cuda):
+    q, k = (torch.randn(6, 2, 64, device=cuda, requires_grad=True) for _ in range(2))
+    pos = torch.arange(6, device=cuda).expand(3, 6).clone()
+    inv, axes = inv_freq(64, 1e4).to(cuda), axis_map((10, 11, 11), device=cuda)
+    op = torch.ops.marathon.rotary_axes
+    for changed in (pos, inv, axes):
+        a, _ = op(q, k, pos, inv, axes)
+        changed.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            a.sum().backward()
+    a, b = op(q, k, pos[0], inv)  # without a table of axes
+    (a.sum() + b.sum()).backward()
+    want, _ = rotary_axes(torch.ones_like(q), None, pos[0], inv, inverse=True)
+    assert torch.equal(q.grad, want)
