@@ -314,8 +314,8 @@ MSHIFT_API int mshift_block_maps(const int32_t* cached_lens, const int32_t* new_
  * negative if `inverse`.  q [n, hq, head_size] and k [n, hk, head_size] of dtype (BF16, F16 or
  * F32) with element strides; the results go to q_out / k_out, which may be q / k
  * themselves but not overlap them otherwise.  axes NULL: axis 0.  The angle is exact
- * modulo a turn to about 2^-24 turns at any position.  An entry of axes outside [0, n_axes)
- * sets MSHIFT_EBIT_TABLE and reads axis 0.
+ * modulo a turn to about 2^-24 turns at any position, for frequencies up to 2^64.  An entry of axes
+ * outside [0, n_axes) sets MSHIFT_EBIT_TABLE and reads axis 0.
  */
 MSHIFT_API int mshift_rotary_axes(int32_t dtype, const void* q, int64_t q_tok, int64_t q_head,
                 void* q_out, int64_t qo_tok, int64_t qo_head, int32_t hq, const void* k,

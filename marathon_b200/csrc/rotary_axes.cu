@@ -8,11 +8,15 @@
 // rotary partners, so a thread holds both halves of its pairs.
 //
 // The angle.  A far position times an fp32 frequency has an fp32 rounding of up to 0.06 rad at a
-// million, so the angle is formed in turns, modulo one, in 64-bit fixed point: inv_freq / 2pi
-// as a fraction of 2^64 is an integer product with the constant 2^64 / 2pi, and position times it
-// wraps modulo 2^64, which is modulo one turn.  What is left, in [-1/2, 1/2) turns, goes to fp32
-// sincospi.  The error is below position * inv_freq * 2^-62 + 2^-24 turns.  One sin and cos a (token,
-// frequency), shared by all heads through shared memory; they cost nothing that shows.
+// million, so the angle is formed in turns, modulo one, in fixed point: inv_freq / 2pi is an integer
+// product with 2^k / 2pi, of which the bits behind the point are kept, and position times those wraps modulo
+// one turn (Payne and Hanek 1983 reduce large arguments so).  What is left, in [-1/2, 1/2) turns, goes to
+// fp32 sincospi.  Positions below 2^31 with frequencies below 32 take 64 bits, which leave an error below 2^-27
+// turns; others take 128 of a product with 2^192 / 2pi: |position| (inv_freq 2^-192 + 2^-128) + 2^-62.  So
+// the fp32 rounding, 2^-25, is the larger part at every 64-bit position for frequencies up to 2^64.  The
+// long form is a call, which costs the short one nothing (the prefill below 128.3 us with and without it;
+// 128 bits for all: 130).  One sin and cos a (token, frequency), shared by
+// all heads through shared memory; they cost nothing that shows.
 //
 // Neighbouring threads have neighbouring vectors, then neighbouring heads, then tokens, so a CTA reads
 // and writes whole rows; one pair of loads a thread at a time, since more
@@ -30,7 +34,8 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 8;      // most tokens of a CTA
 constexpr int kRotMaxHalf = 256;   // frequencies: rotary up to 512
-constexpr uint64_t kTurn = 0x28be60db9391054aull;  // 2^64 / 2pi
+// 2^192 / 2pi, the lowest word first
+constexpr uint64_t kTurn0 = 0x36d8a5664f10e410ull, kTurn1 = 0x7f09d5f47d4d3770ull, kTurn2 = 0x28be60db9391054aull;
 
 struct RotArgs {
   const void* q;
@@ -55,21 +60,34 @@ struct alignas(VEC * sizeof(T)) Pack {
   T x[VEC];
 };
 
-// inv_freq / 2pi turns, modulo one, as a fraction of 2^64.
-__device__ __forceinline__ uint64_t turns_per_position(float inv) {
+// far * m 2^(e - 150) / 2pi turns, modulo one, as a fraction of 2^64, by way of m 2^192 / 2pi in four
+// words, of which the bits from 214 - e on are 128 behind the point.
+__device__ __noinline__ uint64_t far_turns(uint64_t m, int e, uint64_t far) {
+  const uint64_t p0 = m * kTurn0, c0 = __umul64hi(m, kTurn0);
+  const uint64_t p1 = m * kTurn1 + c0, c1 = __umul64hi(m, kTurn1) + (p1 < c0);
+  const uint64_t p2 = m * kTurn2 + c1, p3 = __umul64hi(m, kTurn2) + (p2 < c1);
+  const int from = 214 - e, word = from >> 6, bit = from & 63;
+  auto at = [&](int i) { return i == 0 ? p0 : i == 1 ? p1 : i == 2 ? p2 : i == 3 ? p3 : 0; };
+  const uint64_t w0 = at(word), w1 = at(word + 1), w2 = at(word + 2);
+  const uint64_t lo = w0 >> bit | w1 << 1 << (63 - bit), hi = w1 >> bit | w2 << 1 << (63 - bit);
+  return far * hi + __umul64hi(far, lo);
+}
+
+// position * inv_freq / 2pi turns, modulo one, as a fraction of 2^64.
+__device__ __forceinline__ uint64_t turns(float inv, int64_t position) {
   const uint32_t b = __float_as_uint(inv);
-  const int e = (int)(b >> 23 & 0xff);
-  const uint64_t m = (b & 0x7fffffu) | (e ? 0x800000u : 0u);  // |inv| = m 2^(e - 150)
-  const uint64_t lo = m * kTurn, hi = __umul64hi(m, kTurn);
-  const int right = 150 - (e ? e : 1);
-  uint64_t f;
-  if (right <= 0)
-    f = -right < 64 ? lo << -right : 0;
-  else if (right < 64)
-    f = (lo >> right) | (hi << (64 - right));
-  else
-    f = right < 128 ? hi >> (right - 64) : 0;
-  return b >> 31 ? 0 - f : f;
+  const int e = max((int)(b >> 23 & 0xff), 1);
+  const uint64_t m = (b & 0x7fffffu) | (b & 0x7f800000u ? 0x800000u : 0u);  // |inv| = m 2^(e - 150)
+  const uint64_t far = position < 0 ? 0 - (uint64_t)position : (uint64_t)position;
+  uint64_t t;
+  if (far >> 31 == 0 && e < 132) {
+    const uint64_t lo = m * kTurn2, hi = __umul64hi(m, kTurn2);
+    const int right = 150 - e;
+    t = far * (right < 64 ? lo >> right | hi << (64 - right) : right < 128 ? hi >> (right - 64) : 0);
+  } else {
+    t = far_turns(m, e, far);
+  }
+  return (position < 0) != (b >> 31 != 0) ? 0 - t : t;
 }
 
 template <typename T, int VEC>
@@ -87,9 +105,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_axes_kernel(const RotArgs 
     const int64_t at = axis * a.pos_axis + t0 + tok;
     const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
                                 : static_cast<const int32_t*>(a.positions)[at];
-    const uint64_t turns = (uint64_t)pos * turns_per_position(a.inv_freq[i]);
     float sn, cs;
-    sincospif((float)(int64_t)turns * 0x1p-63f, &sn, &cs);
+    sincospif((float)(int64_t)turns(a.inv_freq[i], pos) * 0x1p-63f, &sn, &cs);
     s_cs[u] = make_float2(cs, sn * a.sign);
   }
   __syncthreads();

@@ -59,9 +59,9 @@ def rotary_axes(
     sign; ``inv_freq`` fp32 ``[rotary / 2]`` with ``rotary <= head_size`` (the tail
     passes through); ``axes`` int32 ``[rotary / 2]`` (:func:`axis_map`), or None where all
     frequencies take axis 0.  NeoX half-split pairs, bf16, fp16 or fp32, rotated in fp32 and
-    rounded once.  Angles are exact modulo a turn to fp32 precision at any position.  Any
-    token and head strides; ``inplace`` writes into ``q`` and ``k`` themselves.  All tensors on one
-    GPU.  An entry of ``axes`` that names no axis is flagged.
+    rounded once.  Angles are exact modulo a turn to fp32 precision at any position (for
+    frequencies up to 2^64).  Any token and head strides; ``inplace`` writes into ``q`` and ``k``
+    themselves.  All tensors on one GPU.  An entry of ``axes`` that names no axis is flagged.
     """
     one = q if q is not None else k
     if one is None:

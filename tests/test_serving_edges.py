@@ -293,3 +293,35 @@ def test_changed_positions_stop_a_rotary_backward(cuda):
     (a.sum() + b.sum()).backward()
     want, _ = rotary_axes(torch.ones_like(q), None, pos[0], inv, inverse=True)
     assert torch.equal(q.grad, want)
+
+
+def _turns(inv, pos, bits=320):
+    """pos * inv / 2 pi modulo one, in integers (pi by Machin's formula)."""
+    one = 1 << bits
+
+    def atan(n):
+        total, term, k = 0, one // n, 1
+        while term:
+            total += term // k if k % 4 == 1 else -(term // k)
+            term //= n * n
+            k += 2
+        return total
+
+    pi = 4 * (4 * atan(5) - atan(239))
+    num, den = float(inv).as_integer_ratio()
+    return (num * pos * one * one // (den * 2 * pi)) % one / one
+
+
+@pytest.mark.gpu
+def test_positions_to_the_ends_of_64_bits(cuda):
+    inv = torch.tensor([1.0, 0.1, 1e-3, 1e-6, 3e-9, 1e-20, 2.0**-126, 1e-42, 1e4, -1e-6, 1e18, 0.0], device=cuda)
+    pos = [1, 2**31 + 3, 2**40 + 1, -(2**48) - 5, 2**55 + 12345, 2**62 + 1, 2**63 - 1, -(2**63), -1]
+    q = torch.zeros(len(pos), 2, 24, device=cuda)
+    q[..., :12] = 1  # a pair (1, 0) turns into (cos, sin)
+    out, _ = rotary_axes(q, None, torch.tensor(pos, device=cuda), inv, check=True)
+    for i, p in enumerate(pos):
+        for j, f in enumerate(inv.tolist()):
+            a = 2 * math.pi * _turns(f, p)
+            for got, want in ((out[i, 0, j], math.cos(a)), (out[i, 0, 12 + j], math.sin(a))):
+                # test_rotary_axes.py's tolerance
+                assert abs(float(got) - want) <= 2.0**-20, (p, f, float(got), want)
