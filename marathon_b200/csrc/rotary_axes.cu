@@ -60,9 +60,10 @@ struct alignas(VEC * sizeof(T)) Pack {
   T x[VEC];
 };
 
-// far * m 2^(e - 150) / 2pi turns, modulo one, as a fraction of 2^64, by way of m 2^192 / 2pi in four
-// words, of which the bits from 214 - e on are 128 behind the point.
-__device__ __noinline__ uint64_t far_turns(uint64_t m, int e, uint64_t far) {
+// far * m 2^(e - 150) / pi half turns, modulo two, by way of m 2^192 / 2pi in four words, of which the bits
+// from 214 - e on are 128 behind the point.  NaN for a frequency that is no number.
+__device__ __noinline__ float far_half_turns(uint64_t m, int e, uint64_t far) {
+  if (e == 255) return __int_as_float(0x7fffffff);
   const uint64_t p0 = m * kTurn0, c0 = __umul64hi(m, kTurn0);
   const uint64_t p1 = m * kTurn1 + c0, c1 = __umul64hi(m, kTurn1) + (p1 < c0);
   const uint64_t p2 = m * kTurn2 + c1, p3 = __umul64hi(m, kTurn2) + (p2 < c1);
@@ -70,24 +71,25 @@ __device__ __noinline__ uint64_t far_turns(uint64_t m, int e, uint64_t far) {
   auto at = [&](int i) { return i == 0 ? p0 : i == 1 ? p1 : i == 2 ? p2 : i == 3 ? p3 : 0; };
   const uint64_t w0 = at(word), w1 = at(word + 1), w2 = at(word + 2);
   const uint64_t lo = w0 >> bit | w1 << 1 << (63 - bit), hi = w1 >> bit | w2 << 1 << (63 - bit);
-  return far * hi + __umul64hi(far, lo);
+  return (float)(int64_t)(far * hi + __umul64hi(far, lo)) * 0x1p-63f;
 }
 
-// position * inv_freq / 2pi turns, modulo one, as a fraction of 2^64.
-__device__ __forceinline__ uint64_t turns(float inv, int64_t position) {
+// position * inv_freq / pi half turns, modulo two.
+__device__ __forceinline__ float half_turns(float inv, int64_t position) {
   const uint32_t b = __float_as_uint(inv);
   const int e = max((int)(b >> 23 & 0xff), 1);
   const uint64_t m = (b & 0x7fffffu) | (b & 0x7f800000u ? 0x800000u : 0u);  // |inv| = m 2^(e - 150)
   const uint64_t far = position < 0 ? 0 - (uint64_t)position : (uint64_t)position;
-  uint64_t t;
+  float t;
   if (far >> 31 == 0 && e < 132) {
     const uint64_t lo = m * kTurn2, hi = __umul64hi(m, kTurn2);
     const int right = 150 - e;
-    t = far * (right < 64 ? lo >> right | hi << (64 - right) : right < 128 ? hi >> (right - 64) : 0);
+    const uint64_t f = right < 64 ? lo >> right | hi << (64 - right) : right < 128 ? hi >> (right - 64) : 0;
+    t = (float)(int64_t)(far * f) * 0x1p-63f;
   } else {
-    t = far_turns(m, e, far);
+    t = far_half_turns(m, e, far);
   }
-  return (position < 0) != (b >> 31 != 0) ? 0 - t : t;
+  return (position < 0) != (b >> 31 != 0) ? -t : t;
 }
 
 template <typename T, int VEC>
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_axes_kernel(const RotArgs 
     const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
                                 : static_cast<const int32_t*>(a.positions)[at];
     float sn, cs;
-    sincospif((float)(int64_t)turns(a.inv_freq[i], pos) * 0x1p-63f, &sn, &cs);
+    sincospif(half_turns(a.inv_freq[i], pos), &sn, &cs);
     s_cs[u] = make_float2(cs, sn * a.sign);
   }
   __syncthreads();

@@ -325,3 +325,13 @@ def test_positions_to_the_ends_of_64_bits(cuda):
             for got, want in ((out[i, 0, j], math.cos(a)), (out[i, 0, 12 + j], math.sin(a))):
                 # test_rotary_axes.py's tolerance
                 assert abs(float(got) - want) <= 2.0**-20, (p, f, float(got), want)
+
+
+@pytest.mark.gpu
+def test_frequencies_that_are_no_numbers(cuda):
+    inv = torch.tensor([1.0, math.inf, math.nan, -math.inf, 0.5], device=cuda)
+    q = torch.randn(3, 2, 12, device=cuda)
+    out, _ = rotary_axes(q, None, torch.tensor([0, 7, -3], device=cuda), inv)
+    bad = torch.tensor([False, True, True, True, False], device=cuda)
+    assert bool(out[..., :5][..., bad].isnan().all()) and bool(out[..., 5:10][..., bad].isnan().all())
+    assert bool(out[..., :5][..., ~bad].isfinite().all()) and torch.equal(out[..., 10:], q[..., 10:])
