@@ -351,7 +351,8 @@ MSHIFT_API int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk,
  * out [rows, hq, head_size] of q's dtype; lse [rows, hq] fp32 (natural log) or NULL.
  * A row that sees no key gets zeros and -inf.  max_query_len / max_seq_len bound the requests'
  * rows and lengths (max_seq_len at most 2^30); a request past them is cut off there and sets
- * MSHIFT_ERR_LENGTHS.  Rows of no request and rows past max_query_len are left as they were, or
+ * MSHIFT_ERR_LENGTHS, as do offsets below zero, out of order or past `rows` (the rows there are
+ * keep their places).  Rows of no request and rows past max_query_len are left as they were, or
  * get zeros and -inf if zero_tail.  Keys in a bad block count as unseen.  Value scales are
  * positive; below 2^-64 they are read as 2^-64.
  * q, out, the cache and workspace start on 16-byte boundaries, as do their rows.

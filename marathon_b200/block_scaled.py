@@ -148,7 +148,8 @@ def attend_block_scaled(
     each other.
 
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
-    the bounds (cut off there), positions past the block table (unseen).
+    the bounds (cut off there), positions past the block table (unseen), offsets below zero, out of order or
+    past the rows of ``q`` (the rows there are keep their places).
     """
     dev = cuda_on("q kv k_scale v_scale block_tables query_start seq_lens out", q, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens, out)

@@ -90,16 +90,19 @@ struct Request {
 
 __device__ __forceinline__ Request request_of(const AttendArgs& a, int r, bool report) {
   Request x;
-  x.q0 = row_start(a.qs, r, a.rows);
-  const int n = max(row_start(a.qs, r + 1, a.rows) - x.q0, 0);
+  const int begin = a.qs[r], end = a.qs[r + 1];
+  x.q0 = min(max(begin, 0), a.rows);
+  const int n = max(min(end, a.rows) - x.q0, 0);
   x.n = min(n, a.max_q);
   x.past = n - x.n;
   const int len = a.lens[r];
-  x.start = (long long)len - n;
+  x.start = len - ((long long)end - x.q0);  // the last row's place is the length's, whether q holds it or not
   const long long held = (long long)a.width * a.bs;
   x.seq = (int)min((long long)min(max(len, 0), a.max_len), held);
   if (report) {
-    if (len > a.max_len || len < 0 || n > a.max_q || x.start < 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+    if (len > a.max_len || len < 0 || n > a.max_q || x.start < 0 || begin < 0 || end < begin ||
+        end > a.rows)
+      flag(a.err, MSHIFT_ERR_LENGTHS);
     if (len > held) flag(a.err, MSHIFT_ERR_POOL);
   }
   return x;

@@ -335,3 +335,22 @@ def test_frequencies_that_are_no_numbers(cuda):
     bad = torch.tensor([False, True, True, True, False], device=cuda)
     assert bool(out[..., :5][..., bad].isnan().all()) and bool(out[..., 5:10][..., bad].isnan().all())
     assert bool(out[..., :5][..., ~bad].isfinite().all()) and torch.equal(out[..., 10:], q[..., 10:])
+
+
+# ------------------------------------------------- offsets that the rows do not hold
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[1, 3, 2], [40, 3, 50]])
+def test_offsets_past_the_rows_are_flagged_and_rows_keep_their_places(cuda, new):
+    take_errors(cuda)
+    c = Case(cuda, [300, 200, 400], new, 4, 2, 128, 16, seed=7)
+    keep = sum(new) - 1
+    for most in (400, 40000):
+        whole, c.dev[0] = c.dev[0], c.dev[0][:keep]
+        got = _attend(c, max_seq_len=most)
+        c.dev[0] = whole
+        assert take_errors(cuda) == _lib.ERR_LENGTHS
+        _check_rows(c, got, list(range(keep)))
+    for qs in ([0, 2, 1, 3], [-1, 0, 0, 1]):
+        c.step[1] = _i32(cuda, qs)
+        _attend(c)
+        assert take_errors(cuda) == _lib.ERR_LENGTHS, qs
