@@ -330,7 +330,8 @@ MSHIFT_API int mshift_rotary_axes(int32_t dtype, const void* q, int64_t q_tok, i
  * their requests' last positions.  A block that holds earlier tokens of its request keeps
  * them (requantised if its scale has to grow); one that does not gets its scale from the
  * new rows alone.  paged->dtype is MSHIFT_E4M3, head_size 64, 128 or 256.  Two requests
- * of a call must not write the same block.
+ * of a call must not write the same block.  Offsets below zero, out of order or past `rows` set
+ * MSHIFT_ERR_LENGTHS (the rows there are keep their places).
  */
 MSHIFT_API int mshift_append_block_scaled(int32_t dtype, const void* k, int64_t k_tok,
                 int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t rows,

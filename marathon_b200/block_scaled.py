@@ -75,7 +75,8 @@ def append_block_scaled(
 
     Rows behind the last request are not written.  No two requests of a call may write the same block
     (copy a shared block before appending to it).  Flagged and skipped: a block outside
-    the cache, positions past the block table, rows before position 0.
+    the cache, positions past the block table, rows before position 0.  Flagged: offsets below zero, out of
+    order or past the rows (the rows there are keep their places).
     """
     dev = cuda_on("k v kv k_scale v_scale block_tables query_start seq_lens", k, v, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens)

@@ -91,15 +91,21 @@ __global__ void __launch_bounds__(kAppWarps * 32) append_kernel(const AppArgs a)
   const int r = find_request(a.reqs, item, [&](int i) {
     return (long long)row_start(a.qs, i, a.rows) / a.bs + 2ll * i;
   });
-  const int q0 = row_start(a.qs, r, a.rows), n = row_start(a.qs, r + 1, a.rows) - q0;
-  if (n <= 0) return;
-  const long long seq = a.lens[r], start = seq - n;
+  const int begin = a.qs[r], end = a.qs[r + 1];
+  const int q0 = min(max(begin, 0), a.rows), n = min(end, a.rows) - q0;
+  if (n <= 0) {
+    if (end != begin && lane == 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+    return;
+  }
+  // the last row's place is the length's, whether the call holds that row or not
+  const long long start = a.lens[r] - ((long long)end - q0), stop = start + n;
   const long long base = (long long)q0 / a.bs + 2ll * r;
   if (item < base) return;
-  if (start < 0 && item == base && lane == 0) flag(a.err, MSHIFT_ERR_LENGTHS);
+  if (item == base && lane == 0 && (start < 0 || begin < 0 || end > a.rows))
+    flag(a.err, MSHIFT_ERR_LENGTHS);
   const long long first = max(start, 0ll);  // rows before position 0 are not written
   const long long col = first / a.bs + (item - base);
-  const long long lo = max(first, col * a.bs), hi = min(seq, (col + 1) * a.bs);
+  const long long lo = max(first, col * a.bs), hi = min(stop, (col + 1) * a.bs);
   if (lo >= hi) return;
   int block = -1;
   if (col < a.width) block = a.tables[(int64_t)r * a.tab_stride + col];

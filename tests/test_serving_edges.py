@@ -12,7 +12,7 @@ import serving
 from marathon_b200 import _lib
 from marathon_b200._serve import geometry
 from marathon_b200.block_maps import block_maps
-from marathon_b200.block_scaled import attend_block_scaled
+from marathon_b200.block_scaled import append_block_scaled, attend_block_scaled
 from marathon_b200.rotary import axis_map, rotary_axes
 from marathon_b200.shift_kernels import inv_freq, take_errors
 from test_block_scaled import NAN_CODE, Case, _cum, _i32
@@ -354,3 +354,22 @@ def test_offsets_past_the_rows_are_flagged_and_rows_keep_their_places(cuda, new)
         c.step[1] = _i32(cuda, qs)
         _attend(c)
         assert take_errors(cuda) == _lib.ERR_LENGTHS, qs
+
+
+@pytest.mark.gpu
+def test_append_with_offsets_past_the_rows(cuda):
+    take_errors(cuda)
+    c = Case(cuda, [40, 37], [9, 12], 2, 2, 64, 16, seed=2, pow2=True)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(21, 2, 64, generator=g).half().to(cuda) for _ in range(2))
+    kv, ks, vs = (x.clone() for x in c.dev[1:])
+    append_block_scaled(k[:18], v[:18], kv, ks, vs, *c.step, 16)
+    assert take_errors(cuda) == _lib.ERR_LENGTHS
+    want = [x.clone() for x in c.dev[1:]]  # the second request's last three rows are not there
+    lens, qs = _i32(cuda, [40, 34]), _i32(cuda, [0, 9, 18])
+    append_block_scaled(k[:18], v[:18], *want, c.step[0], qs, lens, 16, check=True)
+    for a, b in zip((kv, ks, vs), want, strict=True):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for qs in ([0, 9, 4], [-2, 9, 21]):
+        append_block_scaled(k, v, kv, ks, vs, c.step[0], _i32(cuda, qs), c.step[2], 16)
+        assert take_errors(cuda) == _lib.ERR_LENGTHS
