@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ShiftError
@@ -29,10 +30,18 @@ def cuda_on(names: str, *tensors: torch.Tensor | None) -> int:
     return at
 
 
-def refuse_grad(what: str, hint: str) -> None:
-    """These operators record no gradient; a caller who would lose one is told."""
-    if torch.is_grad_enabled():
+def tangents() -> bool:
+    """Whether forward-mode differentiation is on, so that tensors may carry tangents."""
+    return forward_ad._current_level >= 0
+
+
+def refuse_grad(what: str, hint: str, *tensors: torch.Tensor | None) -> None:
+    """These operators record no gradient and carry no tangent; a caller who would lose one is told."""
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         raise ShiftError(f"{what} records no gradient: {hint}")
+    if tangents() and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise ShiftError(f"{what} has no forward-mode gradient: {hint}")
 
 
 def int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> int:

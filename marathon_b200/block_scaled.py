@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from ._serve import (
     block_table_rows, cuda_on, geometry, heads_rows, int32_vector, launch, overlap, refuse_grad,
-    scale_strides,
+    scale_strides, tangents,
 )
 from .paged import dtype_code
 
@@ -80,8 +80,8 @@ def append_block_scaled(
     """
     dev = cuda_on("k v kv k_scale v_scale block_tables query_start seq_lens", k, v, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens)
-    if k.requires_grad or v.requires_grad:
-        refuse_grad("append_block_scaled", "detach k and v")
+    if k.requires_grad or v.requires_grad or k_scale.requires_grad or v_scale.requires_grad or tangents():
+        refuse_grad("append_block_scaled", "detach its arguments", k, v, k_scale, v_scale)
     geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
                              layout)
     code = dtype_code(k.dtype)
@@ -154,8 +154,9 @@ def attend_block_scaled(
     """
     dev = cuda_on("q kv k_scale v_scale block_tables query_start seq_lens out", q, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens, out)
-    if q.requires_grad or (out is not None and out.requires_grad):
-        refuse_grad("attend_block_scaled", "a cache of codes is not trained through")
+    if q.requires_grad or k_scale.requires_grad or v_scale.requires_grad or tangents() or \
+            (out is not None and out.requires_grad):
+        refuse_grad("attend_block_scaled", "a cache of codes is not trained through", q, k_scale, v_scale, out)
     geo, cache, step = _step(kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
                              layout)
     if q.dtype is torch.bfloat16:

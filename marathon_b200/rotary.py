@@ -16,7 +16,7 @@ from collections.abc import Sequence
 import torch
 
 from . import _lib
-from ._serve import cuda_on, heads_rows, int32_vector, launch, overlap, refuse_grad
+from ._serve import cuda_on, heads_rows, int32_vector, launch, overlap, refuse_grad, tangents
 from .paged import dtype_code
 
 __all__ = ["axis_map", "rotary_axes"]
@@ -67,9 +67,9 @@ def rotary_axes(
     if one is None:
         raise _lib.ShiftError("rotary_axes needs q or k")
     dev = cuda_on("q k positions inv_freq axes", q, k, positions, inv_freq, axes)
-    if one.requires_grad or (k is not None and k.requires_grad):
+    if one.requires_grad or (k is not None and k.requires_grad) or inv_freq.requires_grad or tangents():
         refuse_grad("rotary_axes", "its gradient is rotary_axes(..., inverse=True) of the result's, and "
-                    "torch.ops.marathon.rotary_axes records it")
+                    "torch.ops.marathon.rotary_axes records that of q and k", q, k, inv_freq)
     code = dtype_code(one.dtype)
     if code == _lib.E4M3:
         raise _lib.ShiftError("rotary_axes takes bf16, fp16 or fp32")

@@ -39,6 +39,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from ._serve import tangents
 from .block_maps import block_maps
 from .block_scaled import append_block_scaled, attend_block_scaled
 from .paged import KVLayers
@@ -149,6 +150,12 @@ def _(kv, stores, segments, block_tables, block_size, layout) -> None:
 
 
 # ------------------------------------------------------------ serving operators
+def _no_tangents(what: str) -> None:
+    """Tangents end at an operator without a word, and some are out of its sight (``torch.func.jvp``'s)."""
+    if tangents():
+        raise ShiftError(f"torch.ops.marathon.{what} has no forward-mode gradient")
+
+
 @torch.library.custom_op("marathon::block_maps", mutates_args=("block_tables",))
 def _block_maps_op(
     cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -171,8 +178,9 @@ def _rotary_axes_op(
     q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     axes: torch.Tensor | None = None, inverse: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor]:
+    _no_tangents("rotary_axes")
     # detached: gradients are recorded around the operator, not in it
-    return rotary_axes(q.detach(), k.detach(), positions, inv_freq, axes, inverse=inverse)
+    return rotary_axes(q.detach(), k.detach(), positions, inv_freq.detach(), axes, inverse=inverse)
 
 
 @_rotary_axes_op.register_fake
@@ -182,6 +190,8 @@ def _(q, k, positions, inv_freq, axes=None, inverse=False):
 
 def _rotary_axes_setup(ctx, inputs, output) -> None:
     _, _, *tables, ctx.inverse = inputs
+    if tables[1].requires_grad:
+        raise ShiftError("torch.ops.marathon.rotary_axes records no gradient of inv_freq")
     ctx.save_for_backward(*tables)  # a table changed before the backward pass is noticed there
 
 
@@ -200,6 +210,7 @@ def _append_block_scaled_op(
     block_tables: torch.Tensor, query_start: torch.Tensor, seq_lens: torch.Tensor, block_size: int,
     layout: str,
 ) -> None:
+    _no_tangents("append_block_scaled")
     append_block_scaled(k, v, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size,
                         layout)
 
@@ -216,6 +227,7 @@ def _attend_block_scaled_op(
     layout: str, max_query_len: int, max_seq_len: int, scale: float | None = None,
     causal: bool = True, window: int = 0,
 ) -> tuple[torch.Tensor, torch.Tensor]:
+    _no_tangents("attend_block_scaled")
     return attend_block_scaled(
         q, kv, k_scale, v_scale, block_tables, query_start, seq_lens, block_size, layout,
         max_query_len=max_query_len, max_seq_len=max_seq_len, scale=scale, causal=causal,

@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import marathon_b200  # noqa: F401  (registers the operators)
 import serving
@@ -14,7 +15,7 @@ from marathon_b200._serve import geometry
 from marathon_b200.block_maps import block_maps
 from marathon_b200.block_scaled import append_block_scaled, attend_block_scaled
 from marathon_b200.rotary import axis_map, rotary_axes
-from marathon_b200.shift_kernels import inv_freq, take_errors
+from marathon_b200.shift_kernels import ShiftError, inv_freq, take_errors
 from test_block_scaled import NAN_CODE, Case, _cum, _i32
 
 
@@ -373,3 +374,52 @@ def test_append_with_offsets_past_the_rows(cuda):
     for qs in ([0, 9, 4], [-2, 9, 21]):
         append_block_scaled(k, v, kv, ks, vs, c.step[0], _i32(cuda, qs), c.step[2], 16)
         assert take_errors(cuda) == _lib.ERR_LENGTHS
+
+
+# ------------------------------------------------------ gradients that would be lost
+def _dual(t):
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(cuda):
+    c = Case(cuda, [40], [2], 4, 2, 128, 16)
+    q, kv, ks, vs = c.dev
+    k = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=cuda)
+    pos, inv = torch.arange(2, device=cuda), inv_freq(128, 1e4).to(cuda)
+    with forward_ad.dual_level():
+        for call in (lambda: rotary_axes(_dual(q), None, pos, inv),
+                     lambda: rotary_axes(None, _dual(q), pos, inv),
+                     lambda: rotary_axes(q, None, pos, _dual(inv)),
+                     lambda: torch.ops.marathon.rotary_axes(_dual(q), k, pos, inv),
+                     lambda: append_block_scaled(_dual(k), k, kv, ks, vs, *c.step, 16),
+                     lambda: append_block_scaled(k, _dual(k), kv, ks, vs, *c.step, 16),
+                     lambda: attend_block_scaled(_dual(q), kv, ks, vs, *c.step, 16, **c.bounds),
+                     lambda: attend_block_scaled(q, kv, _dual(ks), vs, *c.step, 16, **c.bounds)):
+            with pytest.raises(ShiftError, match="gradient"):
+                call()
+        rotary_axes(q, None, pos, inv)  # nothing to lose
+    for f in (lambda x: torch.ops.marathon.rotary_axes(x, k, pos, inv)[0],
+              lambda x: torch.ops.marathon.attend_block_scaled(x, kv, ks, vs, *c.step, 16, "nhd", 2, 40)[0]):
+        with pytest.raises(ShiftError, match="gradient"):
+            torch.func.jvp(f, (q,), (q,))
+
+
+def _leaf(t):
+    return t.clone().requires_grad_()
+
+
+@pytest.mark.gpu
+def test_gradients_of_frequencies_and_scales_are_refused(cuda):
+    c = Case(cuda, [40], [2], 4, 2, 128, 16)
+    q, kv, ks, vs = c.dev
+    k = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=cuda)
+    pos, inv = torch.arange(2, device=cuda), inv_freq(128, 1e4).to(cuda)
+    for call in (lambda: rotary_axes(q, None, pos, _leaf(inv)),
+                 lambda: torch.ops.marathon.rotary_axes(q, k, pos, _leaf(inv)),
+                 lambda: append_block_scaled(k, k, kv, _leaf(ks), vs, *c.step, 16),
+                 lambda: attend_block_scaled(q, kv, ks, _leaf(vs), *c.step, 16, **c.bounds)):
+        with pytest.raises(ShiftError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
