@@ -84,6 +84,20 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def distinct(t: torch.Tensor) -> bool:
+    """Whether the elements of a tensor that is written lie in different places: its dimensions
+    nest in the order of their strides, each wider than what is inside it."""
+    if t.is_contiguous():
+        return True
+    shape, reach = t.shape, 0
+    for stride, n in sorted(zip(t.stride(), shape, strict=True)):
+        if n > 1:
+            if stride <= reach:
+                return 0 in shape
+            reach += (n - 1) * stride
+    return True
+
+
 def heads_rows(t: torch.Tensor, name: str, written: bool = False) -> tuple[int, int]:
     """(token, head) strides of a ``[tokens, heads, head_size]`` tensor with contiguous heads."""
     stride = t.stride()
@@ -91,8 +105,8 @@ def heads_rows(t: torch.Tensor, name: str, written: bool = False) -> tuple[int, 
         raise ShiftError(f"{name} must be [tokens, heads, head_size], got {tuple(t.shape)}")
     if stride[2] != 1 and t.shape[2] > 1:
         raise ShiftError(f"{name}'s head dimension must be contiguous")
-    if written and 0 in stride and any(n > 1 and s == 0 for n, s in zip(t.shape, stride, strict=True)):
-        raise ShiftError(f"{name} is written and must not repeat its elements")
+    if written and not distinct(t):
+        raise ShiftError(f"{name} is written and must not repeat or overlap its elements")
     return stride[0], stride[1]
 
 

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._serve import (
-    block_table_rows, cuda_on, geometry, heads_rows, int32_vector, launch, overlap, refuse_grad,
+    block_table_rows, cuda_on, distinct, geometry, heads_rows, int32_vector, launch, overlap, refuse_grad,
     scale_strides, tangents,
 )
 from .paged import dtype_code
@@ -97,11 +97,13 @@ def append_block_scaled(
                                   f"{tuple(t.shape)}")
         if at % 16 or tok % vec or head % vec:
             raise _lib.ShiftError(f"{name}'s rows must start on 16-byte boundaries")
-    if 0 in cache[4:6] or 0 in cache[7:9]:
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if any(m > 1 and s == 0 for m, s in zip(t.shape, t.stride(), strict=True)):
-                raise _lib.ShiftError(f"{name} is written and must not repeat its elements")
-    if cache[3] == cache[6] and k_scale.numel():
+    apart = 4 * geo.num_blocks * geo.heads  # bytes of a contiguous scale
+    if not (kv.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        apart = min(apart, 1)
+        for name, t in (("kv", kv), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if not distinct(t):
+                raise _lib.ShiftError(f"{name} is written and must not repeat or overlap its elements")
+    if abs(cache[3] - cache[6]) < apart:
         raise _lib.ShiftError("k_scale and v_scale must be two tensors")
     launch(_lib.load().mshift_append_block_scaled, "append_block_scaled", dev,
            (code, *k_rows, *v_rows, n, *cache, *step), check)

@@ -423,3 +423,33 @@ def test_gradients_of_frequencies_and_scales_are_refused(cuda):
             call()
         with torch.no_grad():
             call()
+
+
+# ------------------------------------------------------------ results in one another
+@pytest.mark.gpu
+def test_results_that_overlap_themselves_are_refused(cuda):
+    c = Case(cuda, [40], [3], 4, 2, 128, 16)
+    q, kv, ks, vs = c.dev
+    buf = torch.zeros(1 << 16, dtype=q.dtype, device=cuda)
+    pos, inv = torch.arange(3, device=cuda), inv_freq(128, 1e4).to(cuda)
+    for strides in ((512, 64, 1), (128, 128, 1), (384, 128, 1), (64, 1024, 1)):
+        o = buf.as_strided((3, 4, 128), strides)
+        with pytest.raises(ShiftError, match="overlap|repeat"):
+            attend_block_scaled(q, kv, ks, vs, *c.step, 16, out=o, **c.bounds)
+        with pytest.raises(ShiftError, match="overlap|repeat"):
+            rotary_axes(o, None, pos, inv, inplace=True)
+    k = torch.zeros(3, 2, 128, dtype=q.dtype, device=cuda)
+    scales = torch.ones(4096, device=cuda)
+    for strides in ((1, 1), (2, 2), (0, 1)):
+        with pytest.raises(ShiftError, match="overlap|repeat"):
+            append_block_scaled(k, k, kv, scales.as_strided(ks.shape, strides), vs, *c.step, 16)
+    n = ks.numel()
+    with pytest.raises(ShiftError, match="two tensors"):
+        append_block_scaled(k, k, kv, scales[:n].view_as(ks), scales[2: n + 2].view_as(ks), *c.step, 16)
+    append_block_scaled(k, k, kv, scales[:n].view_as(ks), scales[n: 2 * n].view_as(ks), *c.step, 16)
+    b8 = torch.zeros(1 << 20, dtype=torch.uint8, device=cuda)
+    for strides in ((512, 512, 256, 1), (8192, 512, 128, 1), (4096, 512, 256, 1)):
+        with pytest.raises(ShiftError, match="overlap"):
+            append_block_scaled(k, k, b8.as_strided(kv.shape, strides), ks, vs, *c.step, 16)
+    for strides in ((512, 128, 1), (128, 512, 1), (4096, 256, 1)):
+        attend_block_scaled(q, kv, ks, vs, *c.step, 16, out=buf.as_strided((3, 4, 128), strides), **c.bounds)
