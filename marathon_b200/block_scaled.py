@@ -178,8 +178,8 @@ def attend_block_scaled(
         raise _lib.ShiftError("max_query_len and window must be non-negative int32s, max_seq_len at most "
                               "2^30 and non-negative")
     scale = head_size ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise _lib.ShiftError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= 2.0**127:  # times log2 e it is an fp32
+        raise _lib.ShiftError(f"scale must be finite and at most 2^127, got {scale}")
     reqs = step[-1]
     lse = None
     zero_tail = out is None

@@ -453,3 +453,11 @@ def test_results_that_overlap_themselves_are_refused(cuda):
             append_block_scaled(k, k, b8.as_strided(kv.shape, strides), ks, vs, *c.step, 16)
     for strides in ((512, 128, 1), (128, 512, 1), (4096, 256, 1)):
         attend_block_scaled(q, kv, ks, vs, *c.step, 16, out=buf.as_strided((3, 4, 128), strides), **c.bounds)
+
+
+@pytest.mark.gpu
+def test_scales_past_fp32_are_refused(cuda):
+    c = Case(cuda, [40], [2], 4, 2, 128, 16)
+    for scale in (1e39, -1e300, 3.4e38):
+        with pytest.raises(ShiftError, match="scale"):
+            c.run(scale=scale)
