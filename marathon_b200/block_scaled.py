@@ -144,10 +144,11 @@ def attend_block_scaled(
     Returns ``out`` (``q``'s type and shape), and with ``return_lse`` the rows' natural-log sums of
     exponentials (fp32 ``[tokens, query heads]``).  A row that sees no key gets zeros and
     ``-inf``.  Rows behind the last request and rows past ``max_query_len`` are left as they were in a
-    given ``out``, and zeros otherwise (lse ``-inf`` either way).  Keys at positions that no row of a tile of rows may see are not
-    read, so stale codes there do no harm, NaN included; a NaN among the values of a token that later rows of the
-    same request see can reach its earlier rows too.
-    Value scales must be positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of
+    given ``out``, and zeros otherwise (lse ``-inf`` either way).  Keys at positions that no row of a tile of
+    rows may see are not read, so stale codes there do no harm, NaN included; a NaN among the values of a
+    token that later rows of the same request see can reach its earlier rows too.  A row whose scores are all
+    NaN gets NaN.  Queries and weights are rounded to f16 for the products, whose sums are fp32; a bf16 result
+    does not show the weights' 2^-11, the error of an fp16 one grows by a fifth.  Value scales must be positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of
     each other.
 
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past

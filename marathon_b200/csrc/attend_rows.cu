@@ -215,11 +215,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// 2^x of a pair without the special-function unit: x = n + f with n the nearest whole number (from
-// adding 1.5 * 2^23, whose low bits then hold n), 2^f by a polynomial of degree 5 fitted here for the
-// least relative error on [-1/2, 1/2] (7.5e-8, 2.3e-7 with fp32's rounding), and n added to its
-// exponent.  Below -126, masked keys' -inf among it, the result is 2^-126, which f16 rounds to zero;
-// NaN stays NaN.
+// 2^x of a pair without the special-function unit, by the textbook reduction: x = n + f with n the nearest
+// whole number (from adding 1.5 * 2^23, whose low bits then hold n), 2^f by a polynomial of degree 5 fitted
+// here for the least relative error on [-1/2, 1/2] (1.6e-7 with its coefficients in fp32, 2.2e-7 with every
+// rounding), and n added to its exponent.  Below -126, masked keys' -inf among it, the result
+// is 2^-126, which f16 rounds to zero; NaN stays NaN.
 __device__ __forceinline__ float2 exp2_pair(float x0, float x1) {
   constexpr float kMagic = 12582912.0f;
   const uint64_t x = pair(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
