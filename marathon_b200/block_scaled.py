@@ -7,7 +7,8 @@ element is ``code * scale[block, head]``.  :func:`append_block_scaled` writes ne
 and chooses the scales; :func:`attend_block_scaled` is the attention that reads the cache, for decoding,
 chunks and whole prefills in one batch.  The codes lie in any of the paged
 layouts of :mod:`marathon_b200.paged` (``nhd``, ``hnd``, ``split``, ``split_blocks``); head sizes 64, 128 and
-256.
+256.  A cache that the shift path filled is read too: its layer's scale, expanded to ``[blocks, heads]``, is
+every block's.
 
 Both take a step as :func:`marathon_b200.block_maps.block_maps` describes it: request ``r`` owns the rows
 ``query_start[r]:query_start[r + 1]``, its last row stands at position ``seq_lens[r] - 1``,
@@ -148,8 +149,8 @@ def attend_block_scaled(
     rows may see are not read, so stale codes there do no harm, NaN included; a NaN among the values of a
     token that later rows of the same request see can reach its earlier rows too.  A row whose scores are all
     NaN gets NaN.  Queries and weights are rounded to f16 for the products, whose sums are fp32; a bf16 result
-    does not show the weights' 2^-11, the error of an fp16 one grows by a fifth.  Value scales must be positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of
-    each other.
+    does not show the weights' 2^-11, the error of an fp16 one grows by a fifth.  Value scales must be
+    positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of each other.
 
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
     the bounds (cut off there), positions past the block table (unseen), offsets below zero, out of order or

@@ -15,7 +15,7 @@ from marathon_b200._serve import geometry
 from marathon_b200.block_maps import block_maps
 from marathon_b200.block_scaled import append_block_scaled, attend_block_scaled
 from marathon_b200.rotary import axis_map, rotary_axes
-from marathon_b200.shift_kernels import ShiftError, inv_freq, take_errors
+from marathon_b200.shift_kernels import ShiftError, inv_freq, rope_shift, scatter_shifted, take_errors
 from test_block_scaled import NAN_CODE, Case, _cum, _i32
 
 
@@ -461,3 +461,35 @@ def test_scales_past_fp32_are_refused(cuda):
     for scale in (1e39, -1e300, 3.4e38):
         with pytest.raises(ShiftError, match="scale"):
             c.run(scale=scale)
+
+
+# --------------------------------------------------------------- beside the shift path
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_a_session_loaded_by_the_shift_path_is_attended(cuda, layout):
+    """Stored rows re-rotated into a paged e4m3 cache with one scale a layer, and a decode step and a chunk over
+    it: the layer's scale is every block's and head's, by strides of zero."""
+    c = Case(cuda, [150, 70], [1, 60], 4, 2, 128, 16, layout=layout, seed=11)
+    c.kv.view(torch.uint8).fill_(NAN_CODE)
+    kv = c.kv.to(cuda)
+    g = torch.Generator().manual_seed(2)
+    rows = (torch.randn(220, 2, 256, generator=g) * 60).clamp(-448, 448).to(torch.float8_e4m3fn).to(cuda)
+    cached = _i32(cuda, [0, 0])
+    m = block_maps(cached, _i32(cuda, c.lens), c.step[0].clone(),
+                   _i32(cuda, [b for t in c.tables for b in t if b >= 0]), _i32(cuda, [0]), 16, 220, check=True)
+    shift = rope_shift(37, 128, inv_freq(128, 1e6), cuda)
+    scatter_shifted(rows, kv, m.slots, 16, layout == "hnd", shift, fp8=True, check=True)
+    k, v = (x.cpu().double() for x in serving.sides(kv, layout))
+    stored = rows[:150].cpu().double()
+    place = [(c.tables[0][p // 16], p % 16) for p in range(150)]
+    turned = serving.rotary(stored[..., :128], torch.full((1, 150), 37), inv_freq(128, 1e6),
+                            torch.zeros(64, dtype=torch.int32), False)
+    for p, (b, o) in enumerate(place):  # the values as they were, the keys turned (within a step of e4m3)
+        assert torch.equal(v[b, o], stored[p, :, 128:])
+        assert bool(((k[b, o] - turned[p].clamp(-448, 448)).abs() <= 2.0**-4 * turned[p].abs() + 2.0**-9).all())
+    ks, vs = torch.tensor(0.021), torch.tensor(0.013)
+    blocks = c.kv.shape[0]
+    c.kv, c.ks, c.vs = kv.cpu(), ks.expand(blocks, 2), vs.expand(blocks, 2)
+    c.dev[1:] = [kv, ks.to(cuda).expand(blocks, 2), vs.to(cuda).expand(blocks, 2)]
+    c.check(c.run())
+    c.check(c.run(max_seq_len=20000))
