@@ -110,6 +110,15 @@ def heads_rows(t: torch.Tensor, name: str, written: bool = False) -> tuple[int, 
     return stride[0], stride[1]
 
 
+def whole_rows(t: torch.Tensor, name: str, vec: int) -> tuple[int, int]:
+    """``heads_rows`` of a tensor some of whose strides are no whole 16-byte vectors of ``vec`` elements:
+    zeros for dimensions of one, whose strides say nothing; else rows do not start on 16-byte boundaries."""
+    tok, head = (s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape[:2], strict=True))
+    if t.data_ptr() % 16 or tok % vec or head % vec:
+        raise ShiftError(f"{name}'s rows must start on 16-byte boundaries")
+    return tok, head
+
+
 _geometries: dict = {}
 
 

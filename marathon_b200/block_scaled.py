@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from ._serve import (
     block_table_rows, cuda_on, distinct, geometry, heads_rows, int32_vector, launch, overlap, refuse_grad,
-    scale_strides, tangents,
+    scale_strides, tangents, whole_rows,
 )
 from .paged import dtype_code
 
@@ -92,12 +92,14 @@ def append_block_scaled(
     want = (n, geo.heads, geo.head_size)
     k_rows, v_rows = (k.data_ptr(), *heads_rows(k, "k")), (v.data_ptr(), *heads_rows(v, "v"))
     vec = 4 if code == _lib.F32 else 8
-    for name, t, (at, tok, head) in (("k", k, k_rows), ("v", v, v_rows)):
+    for name, t in (("k", k), ("v", v)):
         if t.shape != want:
             raise _lib.ShiftError(f"{name} must be [tokens, {geo.heads}, {geo.head_size}], got "
                                   f"{tuple(t.shape)}")
-        if at % 16 or tok % vec or head % vec:
-            raise _lib.ShiftError(f"{name}'s rows must start on 16-byte boundaries")
+    if k_rows[0] % 16 or k_rows[1] % vec or k_rows[2] % vec:
+        k_rows = (k_rows[0], *whole_rows(k, "k", vec))
+    if v_rows[0] % 16 or v_rows[1] % vec or v_rows[2] % vec:
+        v_rows = (v_rows[0], *whole_rows(v, "v", vec))
     apart = 4 * geo.num_blocks * geo.heads  # bytes of a contiguous scale
     if not (kv.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         apart = min(apart, 1)
@@ -175,7 +177,7 @@ def attend_block_scaled(
         raise _lib.ShiftError(f"q {tuple(q.shape)} does not fit {geo.heads} heads of {geo.head_size}")
     q_at = q.data_ptr()
     if q_at % 16 or q_tok % 8 or q_head % 8:
-        raise _lib.ShiftError("q's rows must start on 16-byte boundaries")
+        q_tok, q_head = whole_rows(q, "q", 8)
     if not 0 <= max_query_len < 2**31 or not 0 <= max_seq_len <= 2**30 or not 0 <= window < 2**31:
         raise _lib.ShiftError("max_query_len and window must be non-negative int32s, max_seq_len at most "
                               "2^30 and non-negative")
@@ -202,7 +204,7 @@ def attend_block_scaled(
             raise _lib.ShiftError(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} "
                                   f"{tuple(out.shape)}")
         if out.data_ptr() % 16 or o_tok % 8 or o_head % 8:
-            raise _lib.ShiftError("out's rows must start on 16-byte boundaries")
+            o_tok, o_head = whole_rows(out, "out", 8)
         for name, t in (("q", q), ("kv", kv), ("k_scale", k_scale), ("v_scale", v_scale)):
             if overlap(out, t):
                 raise _lib.ShiftError(f"out shares memory with {name}")

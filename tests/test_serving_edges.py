@@ -463,6 +463,29 @@ def test_scales_past_fp32_are_refused(cuda):
             c.run(scale=scale)
 
 
+@pytest.mark.gpu
+def test_strides_of_single_rows_and_heads_say_nothing(cuda):
+    """One token out of rows of an odd width, one head of an odd stride: 16-byte boundaries all the same."""
+    c = Case(cuda, [40], [1], 4, 1, 128, 16)
+    q, kv, ks, vs = c.dev
+    want = c.run()
+    odd = torch.zeros(1024, dtype=q.dtype, device=cuda)
+    for shape, strides in (((1, 4, 128), (4 * 128 + 3, 128, 1)), ((1, 4, 128), (7, 128, 1))):
+        c.dev[0] = odd.as_strided(shape, strides).copy_(q)
+        got = c.run(out=torch.zeros(1024, dtype=q.dtype, device=cuda).as_strided(shape, strides))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    pos, inv = torch.tensor([7], device=cuda), inv_freq(128, 1e4).to(cuda)
+    assert torch.equal(rotary_axes(c.dev[0], None, pos, inv)[0], rotary_axes(q, None, pos, inv)[0])
+    k = torch.randn(1, 1, 128, device=cuda).to(q.dtype)
+    caches = []
+    for strides in ((128, 128, 1), (5, 3, 1)):
+        cache = [x.clone() for x in (kv, ks, vs)]
+        x = odd.as_strided((1, 1, 128), strides).copy_(k)
+        append_block_scaled(x, x, *cache, *c.step, 16, check=True)
+        caches.append(cache)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*caches, strict=True))
+
+
 # --------------------------------------------------------------- beside the shift path
 @pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["nhd", "hnd"])
