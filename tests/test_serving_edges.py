@@ -295,6 +295,38 @@ def test_changed_positions_stop_a_rotary_backward(cuda):
     want, _ = rotary_axes(torch.ones_like(q), None, pos[0], inv, inverse=True)
     assert torch.equal(q.grad, want)
 
+@pytest.mark.gpu
+def test_a_rotary_step_with_its_backward_replays_from_a_graph(cuda):
+    q = torch.randn(6, 3, 64, device=cuda, requires_grad=True)
+    k = torch.randn(6, 2, 64, device=cuda, requires_grad=True)
+    w = torch.randn(6, 3, 64, device=cuda)
+    pos = torch.randint(0, 900, (3, 6), device=cuda)
+    inv, axes = inv_freq(64, 1e4).to(cuda), axis_map((10, 11, 11), device=cuda)
+
+    def step():
+        a, b = torch.ops.marathon.rotary_axes(q, k, pos, inv, axes)
+        return a.detach(), b.detach(), *torch.autograd.grad((a * w).sum() + b.square().sum(), (q, k))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        with torch.no_grad():
+            q.normal_()
+            k.normal_()
+            w.normal_()
+        pos.random_(0, 900)
+        g.replay()
+        for x, y in zip(got, step(), strict=True):
+            assert torch.equal(x, y)
+
+
 
 def _turns(inv, pos, bits=320):
     """pos * inv / 2 pi modulo one, in integers (pi by Machin's formula)."""
