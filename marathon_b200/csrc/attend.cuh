@@ -19,7 +19,9 @@
 // likewise.  The roundings to fewer than 32 bits are these, of P and of Q, which are what the f16 products
 // ask for (tf32 ones run at half their rate), and the result's own: P's is 2^-11 of each weight, against
 // the result's 2^-8 in bf16 and 2^-11 in fp16 (errors against 64 bits of 1.7e-3 and 2.5e-4; 32-bit weights
-// give 1.7e-3 and 2.1e-4).
+// give 1.7e-3 and 2.1e-4).  Below 2^-14 P is subnormal and off by up to 2^-25 of M's unit: an element to which
+// only keys with such weights contribute, the heavier keys' values being zero there, has that absolute
+// error and no relative one.
 #pragma once
 
 #include "serve_common.cuh"

@@ -20,8 +20,10 @@
 // copies, two steps (8 KB at D = 128) ahead of the one it works on; chunks of 16 bytes are swizzled
 // so that the fragments' reads hit every bank once.
 //
-// 64 sessions of 2k-32k tokens, 32 query heads over 8 of 128: 360-390 us, 5 TB/s, 0.75-0.8 of the
-// copy peak; what is left is issue (some 210 instructions a step, half of them conversions and products).
+// 64 sessions of 2k-32k tokens, 32 query heads over 8 of 128: 358-396 us by the box, 4.8-5.3 TB/s, 0.73-0.81
+// of the copy peak (head size 64: 249, 256: 705; blocks of 24 tokens: 385).  58 % of the issue slots are
+// used, by some 210 instructions a step, half of them conversions and products; the rest of the time a
+// scheduler's four warps wait, each for its own chain.
 // Four stages leave three CTAs an SM instead of four: 447 us; five: 569; the next step's codes in registers
 // instead of the ring: 502; five or six CTAs an SM with spilled registers: 403, 412.
 #include "attend.cuh"
@@ -610,7 +612,8 @@ int few_chunk(int64_t units, int max_len, int64_t bytes) {
 
 // Keys of a split of the many-rows kernel.  One CTA an SM: `units` CTAs a split run in rounds of
 // 148, each as long as its tiles of 128 keys and five more for starting and writing back (a tile takes
-// 2.3 us, both measured).  Splitting fills the last round, and costs the partial results' way to memory and
+// 2.3 us at head size 128, both measured; by the whole kernel's times 2.1 at 64, and 3.6 in blocks that are no
+// multiple of 16).  Splitting fills the last round, and costs the partial results' way to memory and
 // back and the join's launch; the cheapest count is taken.  Measured both ways: 64-244 tokens over eight
 // histories 483 us whole, 506 in three, 457 in four; 1,024 tokens over 16,384 297 us whole, 370 in seven; 244
 // over 30,720 654 us whole, 250-260 in seven to fifteen.

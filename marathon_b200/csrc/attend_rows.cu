@@ -20,12 +20,13 @@
 // 128 t + 64 b, O of tile t at 256 + D t.  O is rescaled in place when a row's maximum passes its
 // reference by 2^8, after the product before has completed; that is rare after the first tiles.
 //
-// What bounds it.  8,192 causal tokens of 32 heads over 8 (550 GFLOP) take 590-600 us, 920 TFLOP/s,
-// 0.56 of cuBLAS's rate.  A half of 64 keys for 256 rows takes about 2,000 cycles; the products need 1,280 of
-// them (50 cycles a 16-deep step of scores, which N = 64 leaves bound by shared memory, 66 of values),
-// the exponentials 770, and the rest is the softmax warps' own latency: two of them a scheduler,
-// in step with each other.  With work left out: products alone 397 us, softmax alone
-// 575, loads alone 383.  Measured and not kept: the row tiles' softmax in turns (618-665 of then
+// What bounds it.  8,192 causal tokens of 32 heads over 8 (550 GFLOP) take 615-645 us by the box, 850-890
+// TFLOP/s, 0.52-0.54 of cuBLAS's rate; of head size 64, whose softmax is the same for half the products,
+// 550; in blocks of 24 tokens, where every key has a scale of its own, 950.  A half of 64 keys for 256
+// rows takes about 2,000 cycles; the products need 1,280 of them (50 cycles a 16-deep step of scores, which
+// N = 64 leaves bound by shared memory, 66 of values), the exponentials 770, and the rest is the softmax
+// warps' own latency: two of them a scheduler, in step with each other.  With work left out: products
+// alone 397 us, softmax alone 575, loads alone 383.  Measured and not kept: the row tiles' softmax in turns (618-665 of then
 // 626), sixteen softmax warps (743), scores given back early with P in columns of its own (668 of 643),
 // all exponentials on the special-function units (626 of 598), 128 keys at once (762 of 693).
 //

@@ -173,7 +173,14 @@ cudaError_t launch_rotary(RotArgs a, cudaStream_t stream) {
                    whole(a.q_out, a.qo_tok, a.qo_head) && whole(a.k_out, a.ko_tok, a.ko_head) &&
                    a.half % kVec == 0 && a.head_size % kVec == 0;
   // one token a CTA, so that a few thousand tokens still give every SM many CTAs; eight, which share
-  // a CTA's start-up, once there are enough for that
+  // a CTA's start-up, once there are enough for that.  In us, one against eight, the launches back to back:
+  //   tokens                     2,048      4,099      8,192     16,384     30,720
+  //   40 + 8 heads of 128, bf16  15 16      27 22      49 40      93 70    169 125
+  //   16 + 8 of 128, fp32, half  19 34      32 39      58 72    109 114    197 171
+  //   8 + 1 of 64, bf16           6  4      11  5      19  7      42 14      79 25
+  //   32 + 8 of 256, fp16        23 25      40 35      72 66    138 114
+  // so the border is late for many rows and early for that fp32 case; two or four tokens a CTA, which no
+  // rule here takes, lie between or below in most of these places
   a.tokens = a.n >= 16384 ? kRotTokens : 1;
   const int v = vec ? kVec : 1;
   const int per = a.half / v + (a.head_size - 2 * a.half) / v;
