@@ -23,7 +23,8 @@ raise.
   ``marathon::attend_block_scaled`` -- the serving operators over a block-scaled e4m3 cache,
   with the arguments of :mod:`marathon_b200.block_maps`, :mod:`~marathon_b200.rotary` and
   :mod:`~marathon_b200.block_scaled`.  ``rotary_axes`` records gradients of ``q`` and ``k``
-  (the rotation by the negative angles).
+  (the rotation by the negative angles).  Rotary, append and attention refuse to run under
+  forward-mode differentiation.
 
 ``stores`` is flat, session-major: session ``s``'s layer ``l`` buffer is
 ``stores[s * n_layers + l]`` (``[capacity, heads, 2*head_size]``).
