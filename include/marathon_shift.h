@@ -355,7 +355,7 @@ MSHIFT_API int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk,
  * MSHIFT_ERR_LENGTHS, as do offsets below zero, out of order or past `rows` (the rows there are
  * keep their places).  Rows of no request and rows past max_query_len are left as they were, or
  * get zeros and -inf if zero_tail.  Keys in a bad block count as unseen.  Value scales are
- * positive; below 2^-64 they are read as 2^-64.
+ * positive; below 2^-64 they are read as 2^-64, and NaN gives NaN to the rows that see it.
  * q, out, the cache and workspace start on 16-byte boundaries, as do their rows.
  */
 MSHIFT_API int mshift_attend_block_scaled(int32_t dtype, const void* q, int64_t q_tok,

@@ -150,7 +150,7 @@ def attend_block_scaled(
     given ``out``, and zeros otherwise (lse ``-inf`` either way).  Keys at positions that no row of a tile of
     rows may see are not read, so stale codes there do no harm, NaN included; a NaN among the values of a
     token that later rows of the same request see can reach its earlier rows too.  A row whose scores are all
-    NaN gets NaN.  Queries and weights are rounded to f16 for the products, whose sums are fp32; a bf16 result
+    NaN gets NaN, and so does one that sees a scale of NaN.  Queries and weights are rounded to f16 for the products, whose sums are fp32; a bf16 result
     does not show the weights' 2^-11, the error of an fp16 one grows by a fifth.  Value scales must be
     positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of each other.
 

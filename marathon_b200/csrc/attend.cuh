@@ -87,6 +87,17 @@ __device__ __forceinline__ int block_column(const AttendArgs& a, int t) {
   return (int)((__umulhi((uint32_t)t, a.bs_mul) + (uint32_t)t) >> a.bs_shift);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// What a value scale adds to the scores and multiplies the weights' sum with.  One below 2^-64 reads as 2^-64;
+// NaN goes to the scores alone, where the rows that do not see the key mask it.
+__device__ __forceinline__ float value_log2(float vs) { return __log2f(max_nan(vs, kScaleFloor)); }
+__device__ __forceinline__ float value_inverse(float vs) { return __frcp_rn(fmaxf(vs, kScaleFloor)); }
+
 // One request's lengths, bounded by what the call's arrays hold.  Rows past the caller's bound have
 // no place in the workspace, which the bound sized: no kernel sees them.
 struct Request {

@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
     return -1;
   };
   // Starts the copies of step st; tokens outside [lo, hi) or in a bad block are zeros, and a bad
-  // block's value scale is -1.
+  // block's value scale is -inf.
   auto fetch = [&](int st, int b) {
     if (st < steps) {
       Stage<D>& x = stage[st / kWarps % kS];
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
         if (b >= 0)
           copy4(to, is_v ? vsh + b * a.vs_blk : ksh + b * a.ks_blk);
         else
-          *to = is_v ? -1.0f : 0.0f;
+          *to = is_v ? -INFINITY : 0.0f;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -274,17 +274,16 @@ __global__ void __launch_bounds__(kWarps * 32) attend_few_kernel(const AttendArg
       }
     }
 
-    // t = S ks rf + log2 vs, masked; a value scale of zero (or below 2^-64) reads as 2^-64
+    // t = S ks rf + log2 vs, masked
     float ks[2], lv[2], rv[2];
     bool good[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int t = PAGE16 ? 0 : g + 8 * e;
       ks[e] = cur.ks[t];
-      good[e] = !(cur.vs[t] < 0.0f);
-      const float vs = fmaxf(cur.vs[t], kScaleFloor);
-      lv[e] = __log2f(vs);
-      rv[e] = __frcp_rn(vs);
+      good[e] = cur.vs[t] != -INFINITY;
+      lv[e] = value_log2(cur.vs[t]);
+      rv[e] = value_inverse(cur.vs[t]);
     }
     const bool whole = __all_sync(0xffffffffu, all_live && t0 >= full_lo && t0 + 16 <= full_hi &&
                                                    good[0] && good[1]);

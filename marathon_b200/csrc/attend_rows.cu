@@ -211,11 +211,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // 2^x of a pair without the special-function unit, by the textbook reduction: x = n + f with n the nearest
 // whole number (from adding 1.5 * 2^23, whose low bits then hold n), 2^f by a polynomial of degree 5 fitted
 // here for the least relative error on [-1/2, 1/2] (1.6e-7 with its coefficients in fp32, 2.2e-7 with every
@@ -349,9 +344,8 @@ __device__ __forceinline__ void finder(const AttendArgs& a, Smem<D>& s, int r, i
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = first + 64 * i, key = sp.first + it * kTile + at, b = b1[i];
-      const float v = fmaxf(vs[i], kScaleFloor);
       s.at[ring][at] = b >= 0 && key >= sp.lo && key < sp.hi ? b * a.blk + (key - block_column(a, key) * a.bs) * a.off : -1ll;
-      s.scale[ring][at] = b >= 0 ? make_float4(ks[i], __log2f(v), __frcp_rn(v), 0.0f)
+      s.scale[ring][at] = b >= 0 ? make_float4(ks[i], value_log2(vs[i]), value_inverse(vs[i]), 0.0f)
                                  : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
     }
     warp_arrive(&s.place_full[ring]);

@@ -175,6 +175,32 @@ def test_rows_whose_only_keys_are_nan(cuda, new, d, most):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("most", [200, 40000])
+@pytest.mark.parametrize("new,d,bs", [(1, 128, 16), (3, 64, 24), (60, 128, 16), (60, 64, 24), (20, 256, 16)])
+def test_value_scales_that_are_nan_or_negative(cuda, new, d, bs, most):
+    """NaN reaches the rows that see a key of its block and no others; below 2^-64 reads as 2^-64."""
+    c = Case(cuda, [200, 90], [new, new], 4, 2, d, bs, seed=8)
+    good = c.run(max_seq_len=most)
+    col = (200 - new // 2 - 1) // bs
+    was = c.dev[3]
+    c.dev[3] = was.clone()
+    c.dev[3][c.tables[0][col], 1] = float("nan")
+    out, lse = c.run(max_seq_len=most)
+    row = torch.arange(2 * new, device=cuda)
+    hit = (row < new) & (200 - new + row >= col * bs)
+    assert bool(hit.any()) and bool(out[hit][:, 2:].isnan().all()) and bool(lse[hit][:, 2:].isnan().all())
+    assert torch.equal(out[~hit], good[0][~hit]) and torch.equal(lse[~hit], good[1][~hit])
+    assert torch.equal(out[:, :2], good[0][:, :2])
+    got = []
+    for scale in (-3.0, 0.0, 2.0**-64):
+        c.dev[3] = was.clone()
+        c.dev[3][c.tables[0][col], 1] = scale
+        got.append(c.run(max_seq_len=most))
+    for out, lse in got[:2]:
+        assert torch.equal(out, got[2][0]) and torch.equal(lse, got[2][1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("most", [64, 40000])
 @pytest.mark.parametrize("new,d", [(1, 128), (40, 128), (40, 64), (4, 256)])
 def test_scores_far_below_zero_are_scores(cuda, new, d, most):
