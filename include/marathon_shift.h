@@ -330,8 +330,8 @@ MSHIFT_API int mshift_rotary_axes(int32_t dtype, const void* q, int64_t q_tok, i
  * their requests' last positions.  A block that holds earlier tokens of its request keeps
  * them (requantised if its scale has to grow); one that does not gets its scale from the
  * new rows alone.  paged->dtype is MSHIFT_E4M3, head_size 64, 128 or 256.  Two requests
- * of a call must not write the same block.  Offsets below zero, out of order or past `rows` set
- * MSHIFT_ERR_LENGTHS (the rows there are keep their places).
+ * of a call must not write the same block.  Offsets past `rows` (those there are keep their places),
+ * below zero or out of order (which of their rows are written is unspecified) set MSHIFT_ERR_LENGTHS.
  */
 MSHIFT_API int mshift_append_block_scaled(int32_t dtype, const void* k, int64_t k_tok,
                 int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t rows,
@@ -352,8 +352,8 @@ MSHIFT_API int64_t mshift_attend_workspace(int32_t rows, int32_t hq, int32_t hk,
  * out [rows, hq, head_size] of q's dtype; lse [rows, hq] fp32 (natural log) or NULL.
  * A row that sees no key gets zeros and -inf.  max_query_len / max_seq_len bound the requests'
  * rows and lengths (max_seq_len at most 2^30); a request past them is cut off there and sets
- * MSHIFT_ERR_LENGTHS, as do offsets below zero, out of order or past `rows` (the rows there are
- * keep their places).  Rows of no request and rows past max_query_len are left as they were, or
+ * MSHIFT_ERR_LENGTHS, as do offsets past `rows` (those there are keep their places), below zero or
+ * out of order (results are unspecified).  Rows of no request and rows past max_query_len are left as they were, or
  * get zeros and -inf if zero_tail.  Keys in a bad block count as unseen.  Value scales are
  * positive; below 2^-64 they are read as 2^-64, and NaN gives NaN to the rows that see it.
  * q, out, the cache and workspace start on 16-byte boundaries, as do their rows.

@@ -76,8 +76,9 @@ def append_block_scaled(
 
     Rows behind the last request are not written.  No two requests of a call may write the same block
     (copy a shared block before appending to it).  Flagged and skipped: a block outside
-    the cache, positions past the block table, rows before position 0.  Flagged: offsets below zero, out of
-    order or past the rows (the rows there are keep their places).
+    the cache, positions past the block table, rows before position 0.  Flagged: offsets past the rows
+    (those there are keep their places), below zero or out of order (which of their rows are written is
+    unspecified).
     """
     dev = cuda_on("k v kv k_scale v_scale block_tables query_start seq_lens", k, v, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens)
@@ -155,8 +156,8 @@ def attend_block_scaled(
     positive (below 2^-64 they are read as 2^-64) and those of a request within 2^96 of each other.
 
     Flagged: a needed block outside the cache (its keys count as unseen), lengths below zero or past
-    the bounds (cut off there), positions past the block table (unseen), offsets below zero, out of order or
-    past the rows of ``q`` (the rows there are keep their places).
+    the bounds (cut off there), positions past the block table (unseen), offsets past the rows of ``q``
+    (those there are keep their places), below zero or out of order (results are unspecified).
     """
     dev = cuda_on("q kv k_scale v_scale block_tables query_start seq_lens out", q, kv, k_scale, v_scale,
                   block_tables, query_start, seq_lens, out)

@@ -109,8 +109,8 @@ struct Request {
 __device__ __forceinline__ Request request_of(const AttendArgs& a, int r, bool report) {
   Request x;
   const int begin = a.qs[r], end = a.qs[r + 1];
-  x.q0 = min(max(begin, 0), a.rows);
-  const int n = max(min(end, a.rows) - x.q0, 0);
+  x.q0 = inside(begin, a.rows);
+  const int n = max(inside(end, a.rows) - x.q0, 0);
   x.n = min(n, a.max_q);
   x.past = n - x.n;
   const int len = a.lens[r];

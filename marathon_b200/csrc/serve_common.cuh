@@ -85,9 +85,10 @@ struct Elem<float> {
   __device__ static float put(float x) { return x; }
 };
 
-// query_start[i], kept inside the call's rows whatever the caller's array holds.
+// An offset kept inside the call's rows, whatever the caller's array holds; and query_start[i] so.
+__device__ __forceinline__ int inside(int offset, int rows) { return min(max(offset, 0), rows); }
 __device__ __forceinline__ int row_start(const int32_t* qs, int i, int rows) {
-  return min(max(qs[i], 0), rows);
+  return inside(qs[i], rows);
 }
 
 // The last r in [0, reqs) with key(r) <= x, for a non-decreasing key (0 if there

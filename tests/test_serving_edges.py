@@ -434,6 +434,36 @@ def test_append_with_offsets_past_the_rows(cuda):
         assert take_errors(cuda) == _lib.ERR_LENGTHS
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [200, 40000])
+def test_offsets_and_lengths_at_the_ends_of_int32(cuda, most):
+    """Nothing is read or written outside the rows, whatever the arrays hold."""
+    low, high = -(2**31), 2**31 - 1
+    c = Case(cuda, [120, 90, 200], [3, 2, 40], 4, 2, 128, 16, seed=9)
+    good = c.run(max_seq_len=most)
+    n = c.q.shape[0]
+    kv, ks, vs = c.dev[1:]
+    k = torch.randn(n, 2, 128, device=cuda).half()
+    wide = torch.full((n + 200, 4, 128), 7.0, dtype=c.q.dtype, device=cuda)
+    for qs in ([0, 3, low, high], [low, 3, 5, high], [0, 3, 5, low], [high, high, low, low], [0, 3, high, 5],
+               [low, low, low, low], [0, 3, 5, -1], [0, 3, 5, high]):
+        for lens in ([120, 90, 200], [120, low, high], [high, high, low]):
+            take_errors(cuda)
+            step = [c.step[0], _i32(cuda, qs), _i32(cuda, lens)]
+            out, lse = attend_block_scaled(*c.dev, *step, 16, return_lse=True, max_query_len=40, max_seq_len=most,
+                                           out=wide[100: 100 + n])
+            assert take_errors(cuda) & _lib.ERR_LENGTHS
+            assert bool((wide[:100] == 7).all()) and bool((wide[100 + n:] == 7).all())
+            if qs == [0, 3, 5, high] and lens[0] == 120:  # in order, only past the rows
+                assert torch.equal(out[:3], good[0][:3]) and torch.equal(lse[:3], good[1][:3])
+            cache = [x.clone() for x in (kv, ks, vs)]
+            append_block_scaled(k, k, *cache, *step, 16)
+            assert take_errors(cuda) & _lib.ERR_LENGTHS
+            free = [b for b in range(ks.shape[0]) if all(b not in t for t in c.tables)]
+            assert torch.equal(cache[0].view(torch.uint8)[free], kv.view(torch.uint8)[free])
+            wide.fill_(7.0)
+
+
 # ------------------------------------------------------ gradients that would be lost
 def _dual(t):
     return forward_ad.make_dual(t, torch.ones_like(t))
